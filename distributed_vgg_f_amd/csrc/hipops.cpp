@@ -35,6 +35,10 @@ std::vector<at::Tensor> dropout_fwd(const at::Tensor&, double, int64_t,
                                     int64_t);
 at::Tensor dropout_bwd(const at::Tensor&, const at::Tensor&, double);
 
+// dropout.hip
+std::vector<at::Tensor> dropout(const at::Tensor&, double, int64_t, int64_t,
+                                const c10::optional<at::Tensor>&);
+
 // lrnpool.hip
 at::Tensor lrn_fwd(const at::Tensor&, int64_t, double, double, double);
 at::Tensor lrn_bwd(const at::Tensor&, const at::Tensor&, int64_t, double,
@@ -86,6 +90,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bump_weight_gen", &dvgg::bump_weight_gen);
   m.def("dropout_fwd", &dvgg::dropout_fwd);
   m.def("dropout_bwd", &dvgg::dropout_bwd);
+  m.def("dropout", &dvgg::dropout, py::arg("x"), py::arg("p"),
+        py::arg("seed"), py::arg("offset"),
+        py::arg("offset_t") = c10::nullopt);
   m.def("lrn_fwd", &dvgg::lrn_fwd);
   m.def("lrn_bwd", &dvgg::lrn_bwd);
   m.def("maxpool_fwd", &dvgg::maxpool_fwd);

@@ -9,6 +9,7 @@
 #include <unordered_map>
 
 #include "common.h"
+#include "philox.h"
 
 namespace dvgg {
 
@@ -250,25 +251,7 @@ void sgd_step(at::Tensor& w32, at::Tensor& wc, const at::Tensor& g,
 }
 
 // ----------------------------------------------------------- dropout K12
-// Philox4x32-10 counter-based RNG: stateless, mask saved as u8.
-DEV void philox_round(u32& c0, u32& c1, u32& c2, u32& c3, u32 k0, u32 k1) {
-  u32 h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0;
-  u32 h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
-  u32 n0 = h1 ^ c1 ^ k0, n1 = l1, n2 = h0 ^ c3 ^ k1, n3 = l0;
-  c0 = n0; c1 = n1; c2 = n2; c3 = n3;
-}
-
-DEV u32x4 philox(u32 lo, u32 hi, u32 key0, u32 key1) {
-  u32 c0 = lo, c1 = hi, c2 = key1, c3 = 0x243F6A88u;
-  u32 k0 = key0, k1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    philox_round(c0, c1, c2, c3, k0, k1);
-    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
-  }
-  return u32x4{c0, c1, c2, c3};
-}
-
+// Mask saved as u8; the form that draws the mask again is in dropout.hip.
 __global__ void dropout_fwd_kernel(const u16* __restrict__ x,
                                    u16* __restrict__ y,
                                    unsigned char* __restrict__ mask, i64 n,

@@ -6,7 +6,7 @@ This is the single seam between the model zoo and the two execution paths.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -42,15 +42,30 @@ def maxpool(x, kernel: int = 3, stride: int = 2, pad: Tuple[int, int] = (0, 0)):
     return cpu_ref.maxpool(x, kernel, stride, pad)
 
 
-def dropout(x, p: float, seed: int = 0, offset: int = 0,
+def dropout(x, p: float, seed: int = 0, offset: Union[int, torch.Tensor] = 0,
             mask: Optional[torch.Tensor] = None):
+    """y = keep * x / (1 - p), p <= 1; p <= 0 returns x itself, p = 1 zeros.
+
+    GPU: bf16, fp16 or fp32 of any shape and strides. The mask is a function
+    of (element index, p, seed, offset), drawn again in the backward pass and
+    never stored; a dropped element is 0 whatever x holds there. seed and
+    offset count modulo 2^32. offset may be one int64 on x's device: a
+    captured graph then draws a new mask at each replay if the caller counts
+    it up. CPU: the mask is torch's own, or the one that is given (`mask` is
+    not read on the GPU).
+    """
     if p <= 0.0:
         return x
+    if not p <= 1.0:
+        raise ValueError(f"dropout: p must not be above 1, got {p}")
+    if p == 1.0:
+        return x.masked_fill(torch.ones((), dtype=torch.bool,
+                                        device=x.device), 0.0)
     if x.is_cuda:
         from .autograd import DropoutFunction
-        return DropoutFunction.apply(x, p, seed, offset)
+        return DropoutFunction.apply(x, float(p), seed, offset)
     if mask is None:
-        gen = torch.Generator().manual_seed(seed + offset)
+        gen = torch.Generator().manual_seed(int(seed + offset))
         mask = (torch.rand(x.shape, generator=gen) >= p).to(x.dtype)
     return cpu_ref.dropout(x, p, mask)
 

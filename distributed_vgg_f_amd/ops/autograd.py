@@ -143,20 +143,26 @@ class MaxPoolFunction(torch.autograd.Function):
 
 
 class DropoutFunction(torch.autograd.Function):
-    """K12: Philox counter-based mask, saved as u8 bitmap."""
+    """K12: Philox counter-based mask that is never stored: backward draws
+    it again from (p, seed, offset) and runs the forward's kernel on dy."""
 
     @staticmethod
-    def forward(ctx, x, p: float, seed: int, offset: int):
-        y, mask = _ext().dropout_fwd(x, p, seed, offset)
-        ctx.save_for_backward(mask)
-        ctx.p = p
+    def forward(ctx, x, p: float, seed: int, offset):
+        ctx.p, ctx.seed, ctx.offset = p, seed, offset
+        if not isinstance(offset, torch.Tensor):
+            return _ext().dropout(x.contiguous(), p, seed, offset)[0]
+        # the kernel keeps a copy of the offset that it drew with: the
+        # caller may count the tensor up before backward runs
+        y, used = _ext().dropout(x.contiguous(), p, seed, 0, offset)
+        ctx.offset = None
+        ctx.save_for_backward(used)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        (mask,) = ctx.saved_tensors
-        dx = _ext().dropout_bwd(dy.contiguous(), mask, ctx.p)
-        return dx, None, None, None
+        offset = ctx.offset if ctx.offset is not None else ctx.saved_tensors[0]
+        return DropoutFunction.apply(dy, ctx.p, ctx.seed, offset), None, \
+            None, None
 
 
 class SoftmaxXentFunction(torch.autograd.Function):
