@@ -20,10 +20,10 @@ BUILD = os.path.join(ROOT, "build", "hipops")
 OUT = os.path.join(ROOT, "distributed_vgg_f_amd", "_hipops.so")
 
 SOURCES = ["gemm_ops.hip", "mem.hip", "lrnpool.hip", "softbn.hip",
-           "dropout.hip",
+           "dropout.hip", "gated.hip",
            "hipops.cpp"]
 HEADERS = ["common.h", "gemm_tile.h", "gemm8.h", "wgrad_fused.h",
-           "philox.h",
+           "philox.h", "mfma_tile.h",
            "conv_ring.h"]
 
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")

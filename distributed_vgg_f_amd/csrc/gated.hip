@@ -1,0 +1,758 @@
+// The gated fully connected unit:
+//
+//   G = X Wg + bg, U = X Wu + bu, H = keep act(G) U / (1 - p)
+//
+// with X [M][K], W [K][N] and the mask of dropout (philox.h). The forward
+// pass is one product whose tiles hold the same columns of G and U, so the
+// activation, the product and the mask are its epilogue. Backward:
+//
+//   dU = keep dH act(G) / (1-p), dG = keep dH U act'(G) / (1-p)
+//   dX = dG Wg^T + dU Wu^T, dWg = X^T dG, dWu = X^T dU, db = column sums
+//
+// one pass over dH, G and U, then two products on the same tiles.
+//
+// Roundings: sums, biases, the activation and the column sums stay in 32
+// bits. G and U are kept for the backward pass, and dG and dU handed to the
+// products, in the type of x: the matrix instructions take 16 bits, and 32
+// would double what the pass between them moves. Each is off by half a step.
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+
+#include "mfma_tile.h"
+#include "philox.h"
+
+namespace dvgg {
+
+static inline hipStream_t cur_stream() {
+  return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+}
+
+DEV float to_f(u16 v, __bf16) { return bf2f(v); }
+DEV float to_f(u16 v, _Float16) {
+  return float(__builtin_bit_cast(_Float16, v));
+}
+DEV u16 from_f(float v, __bf16) { return f2bf(v); }
+DEV u16 from_f(float v, _Float16) {
+  return __builtin_bit_cast(u16, _Float16(v));
+}
+
+// ------------------------------------------------------------- activations
+enum Act { SILU, GELU, GELU_TANH, RELU, SIGMOID };
+
+DEV float sigmoid_f(float z) { return __frcp_rn(1.f + __expf(-z)); }
+
+// act(g) and act'(g). tanh(z) = 2 sigmoid(2z) - 1, so the tanh form of gelu
+// is g sigmoid(2z): nothing cancels. NaN passes through all of them.
+DEV float act_f(int act, float g, float& d) {
+  if (act == RELU) {
+    d = g <= 0.f ? 0.f : 1.f;
+    return g <= 0.f ? 0.f : g;
+  }
+  if (act == GELU) {
+    float c = 0.5f * erfcf(-0.70710678118654752f * g);
+    d = c + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+    return g * c;
+  }
+  if (act == GELU_TANH) {
+    float z2 = 1.5957691216057308f * (g + 0.044715f * g * g * g);
+    float s = sigmoid_f(z2), w = s * (1.f - s);
+    // w is 0 where g * g no longer fits 32 bits
+    d = w > 0.f ? s + g * w * 1.5957691216057308f *
+                          (1.f + 0.134145f * g * g) : s;
+    return g * s;
+  }
+  float s = sigmoid_f(g);
+  if (act == SIGMOID) {
+    d = s * (1.f - s);
+    return s;
+  }
+  d = s * (1.f + g * (1.f - s));
+  return g * s;
+}
+
+// Bits 0..3: which of the 4 elements from flat index i stay. Their block of
+// the generator is one if i is a multiple of 4, else two.
+DEV u32 keep_from(const DropArgs& d, u32 off, i64 i) {
+  u32 sh = u32(i & 3);
+  u32 k = keep4(d, off, i >> 2);
+  if (sh) k = (k | keep4(d, off, (i >> 2) + 1) << 4) >> sh;
+  return k & 15u;
+}
+
+// ---------------------------------------------------------------- epilogue
+struct OutArgs {
+  u16* h;             // [M][N]
+  u16* gu;            // [2][M][ldg] or null
+  const u16* bias[2]; // [N] or null
+  int M, N;
+  i64 ldg;
+  int act;
+  int drop;           // 1: keep/scale by `d`
+  DropArgs d;
+};
+
+// Four columns of one row: g and u without their biases.
+template <class T>
+DEV void finish4(const OutArgs& o, u32 off, int m, int n, f32x4 g, f32x4 u) {
+  u32 keep = o.drop ? keep_from(o.d, off, (i64)m * o.N + n) : 15u;
+  s16x4 hv, gv, uv;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    int c = min(n + r, o.N - 1);
+    float gr = g[r], ur = u[r], d;
+    if (o.bias[0]) gr += to_f(o.bias[0][c], T());
+    if (o.bias[1]) ur += to_f(o.bias[1][c], T());
+    float h = act_f(o.act, gr, d) * ur;
+    if (o.drop) h = (keep >> r & 1) ? h * o.d.scale : 0.f;
+    hv[r] = short(from_f(h, T()));
+    gv[r] = short(from_f(gr, T()));
+    uv[r] = short(from_f(ur, T()));
+  }
+  u16* hp = o.h + (i64)m * o.N + n;
+  if ((o.N & 3) == 0) {
+    *reinterpret_cast<s16x4*>(hp) = hv;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < o.N) hp[r] = u16(hv[r]);
+  }
+  if (o.gu) {         // rows of ldg, a multiple of 8, hold all four
+    u16* gp = o.gu + (i64)m * o.ldg + n;
+    *reinterpret_cast<s16x4*>(gp) = gv;
+    *reinterpret_cast<s16x4*>(gp + (i64)o.M * o.ldg) = uv;
+  }
+}
+
+template <class T>
+DEV void store4(u16* c, int n, int N, f32x4 v) {
+  s16x4 o;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = short(from_f(v[r], T()));
+  if ((N & 3) == 0) {
+    *reinterpret_cast<s16x4*>(c + n) = o;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < N) c[n + r] = u16(o[r]);
+  }
+}
+
+// ---------------------------------------------------------------- products
+// FWD    [M][2N] = X [Wg | Wu]             a tile: 16 FN columns of each
+// DGRAD  [M][K]  = dG Wg^T + dU Wu^T       two parts of the contraction
+// WGRAD  2 x [K][N] = X^T dG, X^T dU       a tile lies in one of the two
+enum Mode { FWD, DGRAD, WGRAD };
+
+struct ProductArgs {
+  const u16* a[2];
+  const u16* b[2];
+  i64 lda, ldb;
+  int rows, cols;       // of one output matrix
+  int k_len;
+  int splits, stages;   // stages of one part of the contraction
+  int tiles_m, tiles_n;
+  float* slab;          // [splits][2 or 1][rows][cols4] if splits > 1
+  i64 slab_ld;          // cols rounded up to 4
+  u16* c[2];            // outputs of DGRAD ([0]) and WGRAD
+  OutArgs out;          // of FWD
+};
+
+// Four columns of each half of a tile's row.
+template <class T, int MODE>
+DEV void emit(const ProductArgs& p, int split, int which, u32 off, int m,
+              int n, int n2, f32x4 v0, f32x4 v1) {
+  if (MODE == FWD) {
+    if (n >= p.cols) return;
+    if (p.splits == 1) {
+      finish4<T>(p.out, off, m, n, v0, v1);
+    } else {
+      float* sp = p.slab + ((i64)split * 2 * p.rows + m) * p.slab_ld + n;
+      *reinterpret_cast<f32x4*>(sp) = v0;
+      *reinterpret_cast<f32x4*>(sp + (i64)p.rows * p.slab_ld) = v1;
+    }
+  } else if (p.splits == 1) {
+    u16* c = (which ? p.c[1] : p.c[0]) + (i64)m * p.cols;
+    if (n < p.cols) store4<T>(c, n, p.cols, v0);
+    if (n2 < p.cols) store4<T>(c, n2, p.cols, v1);
+  } else {
+    constexpr int MATS = MODE == WGRAD ? 2 : 1;
+    float* sp = p.slab +
+        (((i64)split * MATS + which) * p.rows + m) * p.slab_ld;
+    if (n < p.cols) *reinterpret_cast<f32x4*>(sp + n) = v0;
+    if (n2 < p.cols) *reinterpret_cast<f32x4*>(sp + n2) = v1;
+  }
+}
+
+template <class T, int MODE, int FM, int FN>
+__global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
+  constexpr bool ATR = MODE == WGRAD, BTR = MODE != DGRAD;
+  using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN>;
+  // two objects, so that reads of one do not wait for loads into the other
+  __shared__ __attribute__((aligned(1024))) char even[TL::STAGE];
+  __shared__ __attribute__((aligned(1024))) char odd[TL::STAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // neighbours on one XCD share panels: tiles run down groups of 8 rows
+  u32 id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int split = __builtin_amdgcn_readfirstlane(id / tiles);
+  int t = id - split * tiles;
+  const int group = 8 * p.tiles_n;
+  const int g0 = t / group * 8, gs = min(8, p.tiles_m - g0);
+  t %= group;
+  const int m0 = __builtin_amdgcn_readfirstlane((g0 + t % gs) * TL::BM);
+  int tn = __builtin_amdgcn_readfirstlane(t / gs);
+  // WGRAD: the second half of the tile columns belongs to dU
+  const int which = MODE == WGRAD && tn >= p.tiles_n / 2;
+  if (which) tn -= p.tiles_n / 2;
+  const int n0 = tn * (MODE == FWD ? TL::HALF : TL::BN);
+
+  TileSrc s;
+  s.lda = u32(p.lda);
+  s.ldb = u32(p.ldb);
+  s.rows_a = p.rows - m0;
+  s.rows_b[0] = p.cols - n0;
+  s.rows_b[1] = MODE == FWD ? p.cols - n0 : p.cols - n0 - TL::HALF;
+  const i64 am = ATR ? m0 : (i64)m0 * p.lda;
+  const i64 bn = BTR ? n0 : (i64)n0 * p.ldb;
+  const i64 bh = BTR ? TL::HALF : (i64)TL::HALF * p.ldb;
+  s.a[0] = p.a[0] + am;
+  s.a[1] = p.a[MODE == DGRAD] + am;
+  if (MODE == FWD) {
+    s.b[0][0] = s.b[1][0] = p.b[0] + bn;
+    s.b[0][1] = s.b[1][1] = p.b[1] + bn;
+  } else {
+    s.b[0][0] = (which ? p.b[1] : p.b[0]) + bn;
+    s.b[0][1] = s.b[0][0] + bh;
+    s.b[1][0] = p.b[1] + bn;
+    s.b[1][1] = s.b[1][0] + bh;
+  }
+  const int q = p.stages / p.splits, r = p.stages % p.splits;
+  s.k_first = (split * q + min(split, r)) * TILE_BK;
+  s.k_last = min(s.k_first + (q + (split < r)) * TILE_BK, p.k_len);
+
+  f32x4 acc[FM][FN];
+  TL tile;
+  tile.run((lds_char*)even, (lds_char*)odd, s, wave, lane, acc);
+
+  // Through LDS, 32 rows of a wave at a time: the lanes then hold whole
+  // stretches of 64 columns of a row (128 bytes a store), and one copy of the
+  // epilogue's code per 32 rows is enough.
+  constexpr int PITCH = 16 * FN + 4;      // floats; + 4: rows change banks
+  static_assert(32 * PITCH * 4 <= TL::STAGE / 2, "a wave's part of a stage");
+  float* mine = reinterpret_cast<float*>(
+      (wave & 2 ? odd : even) + (wave & 1) * (TL::STAGE / 2));
+  __syncthreads();
+  const u32 off = MODE == FWD && p.out.drop ? p.out.d.off() : 0;
+  const int nw = n0 + (wave & 1) * 8 * FN;
+#pragma unroll
+  for (int i = 0; i < FM; i += 2) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        *reinterpret_cast<f32x4*>(mine + (q * 16 + (lane & 15)) * PITCH +
+                                  j * 16 + (lane >> 4) * 4) = acc[i + q][j];
+    // one wave writes and reads: its LDS instructions keep their order
+    const int mw = m0 + (wave >> 1) * 16 * FM + i * 16;
+    constexpr int CH = 2 * FN;            // 4-column chunks of a half row
+#pragma unroll 1
+    for (int c = lane; c < 32 * CH; c += 64) {
+      const int m = mw + c / CH, n = nw + c % CH * 4;
+      const float* v = mine + c / CH * PITCH + c % CH * 4;
+      f32x4 v0 = *reinterpret_cast<const f32x4*>(v);
+      f32x4 v1 = *reinterpret_cast<const f32x4*>(v + 8 * FN);
+      if (m >= p.rows) break;
+      emit<T, MODE>(p, split, which, off, m, n, n + TL::HALF, v0, v1);
+    }
+  }
+}
+
+// ------------------------------------------------- joining a split product
+// Sums the slabs in their order (the same result every time), 4 columns a
+// thread.
+template <class T>
+__global__ __launch_bounds__(256) void join_gated_kernel(
+    const float* __restrict__ slab, int splits, i64 slab_ld, OutArgs o) {
+  const u32 off = o.drop ? o.d.off() : 0;
+  const int cols4 = int(slab_ld / 4);
+  const i64 one = (i64)o.M * slab_ld;
+  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < (i64)o.M * cols4;
+       c += (i64)gridDim.x * 256) {
+    const float* sp = slab + c * 4;
+    f32x4 g{0.f, 0.f, 0.f, 0.f}, u = g;
+    for (int s = 0; s < splits; ++s) {
+      g += *reinterpret_cast<const f32x4*>(sp);
+      u += *reinterpret_cast<const f32x4*>(sp + one);
+      sp += 2 * one;
+    }
+    int m = int(c / cols4);
+    finish4<T>(o, off, m, int(c - (i64)m * cols4) * 4, g, u);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void join_plain_kernel(
+    const float* __restrict__ slab, int splits, i64 slab_ld, int rows,
+    int cols, int mats, u16* c0, u16* c1) {
+  const int cols4 = int(slab_ld / 4);
+  const i64 one = (i64)rows * slab_ld * mats;
+  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x;
+       c < (i64)rows * mats * cols4; c += (i64)gridDim.x * 256) {
+    const float* sp = slab + c * 4;
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s, sp += one)
+      v += *reinterpret_cast<const f32x4*>(sp);
+    i64 m = c / cols4;
+    int n = int(c - m * cols4) * 4;
+    u16* out = m < rows ? c0 + m * cols : c1 + (m - rows) * cols;
+    store4<T>(out, n, cols, v);
+  }
+}
+
+// ------------------------------------------- between dH and the products
+// dG and dU (rows of ldg, zeros behind N) and, if `part` is given, the sums
+// of each block's rows: part [gridDim.y][2][ldg]. A thread takes 8 columns,
+// a block 256, its 8 groups of 32 threads every eighth row.
+struct MidArgs {
+  const u16* dh;
+  i64 ldh;
+  const u16* gu;
+  u16* dgu;
+  float* part;
+  int M, N;
+  i64 ldg;
+  int rows_per_block;
+  int act, drop;
+  DropArgs d;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
+  __shared__ float red[8][2][256];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = blockIdx.x * 256 + tx * 8;
+  const u32 off = a.drop ? a.d.off() : 0;
+  float sg[8] = {}, su[8] = {};
+  const int r0 = blockIdx.y * a.rows_per_block;
+  const int r1 = min(a.M, r0 + a.rows_per_block);
+  const bool wide = (a.N & 7) == 0 && (a.ldh & 7) == 0 &&
+                    (reinterpret_cast<uintptr_t>(a.dh) & 15) == 0;
+  if (n < a.ldg) {
+    for (int m = r0 + ty; m < r1; m += 8) {
+      const u16* gp = a.gu + (i64)m * a.ldg + n;
+      s16x8 g = *reinterpret_cast<const s16x8*>(gp);
+      s16x8 u = *reinterpret_cast<const s16x8*>(gp + (i64)a.M * a.ldg);
+      s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
+      const u16* hp = a.dh + (i64)m * a.ldh + n;
+      if (wide) {
+        h = *reinterpret_cast<const s16x8*>(hp);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + j < a.N) h[j] = short(hp[j]);
+      }
+      u32 keep = 255u;
+      if (a.drop) {
+        i64 i = (i64)m * a.N + n;
+        keep = keep_from(a.d, off, i) | keep_from(a.d, off, i + 4) << 4;
+      }
+      s16x8 og, ou;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float d, v = to_f(u16(h[j]), T());
+        float act = act_f(a.act, to_f(u16(g[j]), T()), d);
+        if (a.drop) v *= a.d.scale;
+        float dg = v * to_f(u16(u[j]), T()) * d, du = v * act;
+        // what was dropped, or lies behind N, passes nothing on
+        if (!(keep >> j & 1) || n + j >= a.N) dg = du = 0.f;
+        sg[j] += dg;
+        su[j] += du;
+        og[j] = short(from_f(dg, T()));
+        ou[j] = short(from_f(du, T()));
+      }
+      u16* op = a.dgu + (i64)m * a.ldg + n;
+      *reinterpret_cast<s16x8*>(op) = og;
+      *reinterpret_cast<s16x8*>(op + (i64)a.M * a.ldg) = ou;
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    red[ty][0][tx * 8 + j] = sg[j];
+    red[ty][1][tx * 8 + j] = su[j];
+  }
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.ldg) return;
+  float vg = 0.f, vu = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    vg += red[r][0][threadIdx.x];
+    vu += red[r][1][threadIdx.x];
+  }
+  float* pp = a.part + (i64)blockIdx.y * 2 * a.ldg + c;
+  pp[0] = vg;
+  pp[a.ldg] = vu;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void bias_join_kernel(
+    const float* __restrict__ part, int blocks, int N, i64 ldg, u16* dbg,
+    u16* dbu) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= N) return;
+  u16* out = blockIdx.y ? dbu : dbg;
+  if (!out) return;
+  part += blockIdx.y * ldg + c;
+  float v = 0.f;
+  for (int b = 0; b < blocks; ++b) v += part[(i64)b * 2 * ldg];
+  out[c] = from_f(v, T());
+}
+
+// -------------------------------------------------------------- rows apart
+// Copies rows of any length and alignment to rows of whole vectors, zeros
+// behind them: what the tiles cannot load goes through here once a call.
+__global__ __launch_bounds__(256) void pad_rows_kernel(
+    const u16* __restrict__ in, i64 sr, i64 sc, u16* __restrict__ out,
+    i64 rows, int cols, int ld) {
+  const int per = ld / 8;
+  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < rows * per;
+       c += (i64)gridDim.x * 256) {
+    i64 r = c / per;
+    int n = int(c - r * per) * 8;
+    s16x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = n + j < cols ? short(in[r * sr + (n + j) * sc]) : short(0);
+    *reinterpret_cast<s16x8*>(out + c * 8) = v;
+  }
+}
+
+// ==================================================================== host
+static i64 up(i64 v, i64 to) { return (v + to - 1) / to * to; }
+
+static const u16* cptr(const at::Tensor& t) {
+  return reinterpret_cast<const u16*>(t.data_ptr());
+}
+static u16* mptr(const at::Tensor& t) {
+  return reinterpret_cast<u16*>(t.data_ptr());
+}
+
+// A matrix that the tiles can load: unit column stride, rows that start on
+// 16 bytes and whose last vector may be read whole.
+static at::Tensor loadable(const at::Tensor& t) {
+  i64 rows = t.size(0), cols = t.size(1);
+  bool ok = t.stride(1) == 1 && cols % 8 == 0 &&
+            (rows == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= cols)) &&
+            reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  if (ok) return t;
+  auto out = at::empty({rows, up(cols, 8)}, t.options());
+  i64 chunks = out.numel() / 8;
+  if (chunks)
+    hipLaunchKernelGGL(pad_rows_kernel,
+                       dim3(u32(std::min<i64>((chunks + 255) / 256, 8192))),
+                       dim3(256), 0, cur_stream(), cptr(t), t.stride(0),
+                       t.stride(1), mptr(out), rows, int(cols),
+                       int(out.size(1)));
+  return out;
+}
+// a single row may carry any stride
+static i64 ld_of(const at::Tensor& t) {
+  return t.size(0) == 1 ? t.size(1) : t.stride(0);
+}
+
+struct Plan { int fm, fn, splits, tiles_m, tiles_n, stages; };
+
+static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
+  Plan p;
+  p.fm = rows > 128 ? 8 : rows > 64 ? 4 : 2;
+  p.fn = 8;
+  p.stages = ceil_div(k_len, TILE_BK);
+  p.tiles_m = ceil_div(rows, 32 * p.fm);
+  p.tiles_n = ceil_div(cols, mode == FWD ? 16 * p.fn : 32 * p.fn) *
+              (mode == WGRAD ? 2 : 1);
+  i64 tiles = (i64)p.tiles_m * p.tiles_n;
+  p.splits = 1;
+  while (tiles * p.splits * 2 <= 256 && p.stages / (p.splits * 2) >= 8)
+    p.splits *= 2;
+  return p;
+}
+
+template <class T, int MODE>
+static void launch(const Plan& pl, const ProductArgs& a) {
+  dim3 grid(u32(pl.tiles_m) * pl.tiles_n * pl.splits);
+  auto st = cur_stream();
+  if (pl.fm == 8)
+    hipLaunchKernelGGL((product_kernel<T, MODE, 8, 8>), grid, dim3(256), 0,
+                       st, a);
+  else if (pl.fm == 4)
+    hipLaunchKernelGGL((product_kernel<T, MODE, 4, 8>), grid, dim3(256), 0,
+                       st, a);
+  else
+    hipLaunchKernelGGL((product_kernel<T, MODE, 2, 8>), grid, dim3(256), 0,
+                       st, a);
+  HIP_CHECK(hipGetLastError());
+}
+
+template <int MODE>
+static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
+                    const at::TensorOptions& opt) {
+  a.splits = pl.splits;
+  a.stages = pl.stages;
+  a.tiles_m = pl.tiles_m;
+  a.tiles_n = pl.tiles_n;
+  a.slab_ld = up(a.cols, 4);
+  const int mats = MODE == DGRAD ? 1 : 2;
+  at::Tensor slab;
+  if (pl.splits > 1) {
+    slab = at::empty({(i64)pl.splits * mats * a.rows * a.slab_ld},
+                     opt.dtype(at::kFloat));
+    a.slab = slab.data_ptr<float>();
+  }
+  const bool half = type == at::kHalf;
+  if (half) launch<_Float16, MODE>(pl, a);
+  else launch<__bf16, MODE>(pl, a);
+  if (pl.splits == 1) return;
+  i64 chunks = (i64)a.rows * (MODE == WGRAD ? 2 : 1) * a.slab_ld / 4;
+  dim3 grid(u32(std::min<i64>((chunks + 255) / 256, 8192)));
+  auto st = cur_stream();
+  if (MODE == FWD) {
+    if (half)
+      hipLaunchKernelGGL(join_gated_kernel<_Float16>, grid, dim3(256), 0, st,
+                         a.slab, pl.splits, a.slab_ld, a.out);
+    else
+      hipLaunchKernelGGL(join_gated_kernel<__bf16>, grid, dim3(256), 0, st,
+                         a.slab, pl.splits, a.slab_ld, a.out);
+  } else if (half) {
+    hipLaunchKernelGGL(join_plain_kernel<_Float16>, grid, dim3(256), 0, st,
+                       a.slab, pl.splits, a.slab_ld, a.rows, a.cols, mats,
+                       a.c[0], a.c[1]);
+  } else {
+    hipLaunchKernelGGL(join_plain_kernel<__bf16>, grid, dim3(256), 0, st,
+                       a.slab, pl.splits, a.slab_ld, a.rows, a.cols, mats,
+                       a.c[0], a.c[1]);
+  }
+  HIP_CHECK(hipGetLastError());
+}
+
+static void check_operand(const at::Tensor& t, const char* name,
+                          const at::Tensor& x, i64 rows, i64 cols) {
+  TORCH_CHECK(t.device() == x.device(), "gated_linear: ", name, " is on ",
+              t.device(), ", x on ", x.device());
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), "gated_linear: ", name,
+              " is ", t.scalar_type(), ", x is ", x.scalar_type());
+  bool shape = rows < 0 ? t.dim() == 1 && t.size(0) == cols
+                        : t.dim() == 2 && t.size(0) == rows &&
+                              t.size(1) == cols;
+  TORCH_CHECK(shape, "gated_linear: ", name, " has shape ", t.sizes(),
+              " instead of ",
+              rows < 0 ? std::to_string(cols)
+                       : std::to_string(rows) + " x " + std::to_string(cols));
+}
+
+static DropArgs gated_drop(const at::Tensor& x, double p, int64_t seed,
+                           int64_t offset,
+                           const c10::optional<at::Tensor>& offset_t) {
+  if (offset_t)
+    TORCH_CHECK(offset_t->device() == x.device() &&
+                offset_t->scalar_type() == at::kLong &&
+                offset_t->numel() == 1,
+                "gated_linear: offset must be one int64 on x's device");
+  return drop_args(p, seed, offset,
+                   offset_t ? reinterpret_cast<const i64*>(
+                                  offset_t->data_ptr<int64_t>())
+                            : nullptr);
+}
+
+__global__ void copy_offset_kernel(const i64* in, i64* out) { *out = *in; }
+
+// Returns h [M][N], and with `train` also what backward wants: G and U as
+// one [2][M][N up to a vector], the three operands as the tiles load them,
+// and the offset that the mask was drawn with if it came from the device.
+std::vector<at::Tensor> gated_fwd(
+    const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
+    const c10::optional<at::Tensor>& bg, const c10::optional<at::Tensor>& bu,
+    int64_t act, double p, int64_t seed, int64_t offset,
+    const c10::optional<at::Tensor>& offset_t, bool train) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "gated_linear: x must be a GPU "
+              "matrix");
+  auto type = x.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf,
+              "gated_linear: x must be bf16 or fp16 on the GPU, got ", type);
+  const i64 M = x.size(0), K = x.size(1);
+  TORCH_CHECK(wg.dim() == 2, "gated_linear: w_gate must be a matrix");
+  const i64 N = wg.size(1);
+  check_operand(wg, "w_gate", x, K, N);
+  check_operand(wu, "w_up", x, K, N);
+  if (bg) check_operand(*bg, "bias_gate", x, -1, N);
+  if (bu) check_operand(*bu, "bias_up", x, -1, N);
+  TORCH_CHECK(K > 0 && N > 0, "gated_linear: K and N must not be 0");
+  TORCH_CHECK(act >= 0 && act <= SIGMOID, "gated_linear: unknown activation");
+  TORCH_CHECK(p >= 0.0 && p < 1.0, "gated_linear: p must lie in [0, 1)");
+  TORCH_CHECK(M < (1 << 30) && K < (1 << 21) && N < (1 << 21),
+              "gated_linear: at most 2^30 rows and 2^21 columns");
+  c10::DeviceGuard guard(x.device());
+  DropArgs d = gated_drop(x, p, seed, offset, offset_t);
+  auto h = at::empty({M, N}, x.options());
+  at::Tensor gu, used;
+  const i64 ldg = up(N, 8);
+  if (train) gu = at::empty({2, M, ldg}, x.options());
+  if (train && offset_t) {
+    used = at::empty({1}, offset_t->options());
+    hipLaunchKernelGGL(copy_offset_kernel, dim3(1), dim3(1), 0, cur_stream(),
+                       d.offset_ptr,
+                       reinterpret_cast<i64*>(used.data_ptr<int64_t>()));
+  }
+  auto xl = loadable(x), gl = loadable(wg);
+  auto ul = loadable(wu);
+  if (ld_of(ul) != ld_of(gl)) {           // one pitch for both
+    gl = gl.contiguous();
+    ul = ul.contiguous();
+  }
+  TORCH_CHECK(ld_of(xl) < (1 << 21) && ld_of(gl) < (1 << 21),
+              "gated_linear: row strides must stay below 2^21");
+  at::Tensor bgc, buc;
+  if (bg) bgc = bg->contiguous();
+  if (bu) buc = bu->contiguous();
+  if (M > 0) {
+    ProductArgs a{};
+    a.a[0] = a.a[1] = cptr(xl);
+    a.b[0] = cptr(gl);
+    a.b[1] = cptr(ul);
+    a.lda = ld_of(xl);
+    a.ldb = ld_of(gl);
+    a.rows = int(M);
+    a.cols = int(N);
+    a.k_len = int(K);
+    a.out = OutArgs{mptr(h), train ? mptr(gu) : nullptr,
+                    {bg ? cptr(bgc) : nullptr, bu ? cptr(buc) : nullptr},
+                    int(M), int(N), ldg, int(act), p > 0.0, d};
+    product<FWD>(type, make_plan(FWD, M, N, K), a, x.options());
+  }
+  if (!train) return {h};
+  std::vector<at::Tensor> r{h, gu, xl, gl, ul};
+  if (used.defined()) r.push_back(used);
+  return r;
+}
+
+// x, wg, wu as gated_fwd returned them; K, N: their true column counts.
+// need: bits dx, dWg, dWu, dbg, dbu. *_out: where the caller wants them.
+std::vector<at::Tensor> gated_bwd(
+    const at::Tensor& dh_, const at::Tensor& gu, const at::Tensor& x,
+    const at::Tensor& wg, const at::Tensor& wu, int64_t K, int64_t N,
+    int64_t act, double p, int64_t seed, int64_t offset,
+    const c10::optional<at::Tensor>& offset_t, int64_t need,
+    const std::vector<c10::optional<at::Tensor>>& outs) {
+  const i64 M = x.size(0), ldg = gu.size(2);
+  auto type = x.scalar_type();
+  TORCH_CHECK(dh_.device() == x.device() && dh_.scalar_type() == type &&
+              dh_.dim() == 2 && dh_.size(0) == M && dh_.size(1) == N,
+              "gated_linear: bad gradient");
+  c10::DeviceGuard guard(x.device());
+  auto opt = x.options();
+  auto dh = dh_.stride(1) == 1 ? dh_ : dh_.contiguous();
+  DropArgs d = gated_drop(x, p, seed, offset, offset_t);
+  const i64 shapes[5][2] = {{M, K}, {K, N}, {K, N}, {1, N}, {1, N}};
+  std::vector<at::Tensor> grads(5), result(5);
+  for (int i = 0; i < 5; ++i) {
+    if (!(need >> i & 1)) continue;
+    auto& out = outs[i];
+    if (out)
+      TORCH_CHECK(out->is_contiguous() && out->device() == x.device() &&
+                  out->numel() == shapes[i][0] * shapes[i][1],
+                  "gated_linear: bad gradient buffer");
+    // a buffer of another type is filled by a copy at the end
+    bool direct = out && out->scalar_type() == type;
+    grads[i] = direct ? *out
+                      : at::empty({shapes[i][0], shapes[i][1]}, opt);
+    result[i] = out ? *out : i < 3 ? grads[i] : grads[i].view({N});
+  }
+  auto ptr = [&](int i) { return grads[i].defined() ? mptr(grads[i]) : nullptr; };
+  if (M == 0) {
+    for (auto& g : grads) if (g.defined()) g.zero_();
+  } else {
+    auto dgu = at::empty_like(gu);
+    const bool bias = (need & 24) != 0;
+    MidArgs a{};
+    a.dh = cptr(dh);
+    a.ldh = M == 1 ? N : dh.stride(0);
+    a.gu = cptr(gu);
+    a.dgu = mptr(dgu);
+    a.M = int(M);
+    a.N = int(N);
+    a.ldg = ldg;
+    a.act = int(act);
+    a.drop = p > 0.0;
+    a.d = d;
+    const int bx = ceil_div(ldg, 256);
+    // about 2048 blocks; 8 rows a turn
+    a.rows_per_block = int(std::max<i64>(8, up(ceil_div(M * bx, 2048), 8)));
+    const int by = ceil_div(M, a.rows_per_block);
+    at::Tensor part;
+    if (bias) {
+      part = at::empty({by, 2, ldg}, opt.dtype(at::kFloat));
+      a.part = part.data_ptr<float>();
+    }
+    const bool half = type == at::kHalf;
+    auto st = cur_stream();
+    TORCH_CHECK(by < 65536, "gated_linear: too many rows");
+    if (half)
+      hipLaunchKernelGGL(mid_kernel<_Float16>, dim3(bx, by), dim3(256), 0, st,
+                         a);
+    else
+      hipLaunchKernelGGL(mid_kernel<__bf16>, dim3(bx, by), dim3(256), 0, st,
+                         a);
+    if (bias) {
+      dim3 g(ceil_div(N, 256), 2);
+      if (half)
+        hipLaunchKernelGGL(bias_join_kernel<_Float16>, g, dim3(256), 0, st,
+                           a.part, by, int(N), ldg, ptr(3), ptr(4));
+      else
+        hipLaunchKernelGGL(bias_join_kernel<__bf16>, g, dim3(256), 0, st,
+                           a.part, by, int(N), ldg, ptr(3), ptr(4));
+    }
+    HIP_CHECK(hipGetLastError());
+    const u16* dg = cptr(dgu);
+    const u16* du = dg + M * ldg;
+    if (need & 1) {
+      ProductArgs q{};
+      q.a[0] = dg;
+      q.a[1] = du;
+      q.b[0] = cptr(wg);
+      q.b[1] = cptr(wu);
+      q.lda = ldg;
+      q.ldb = ld_of(wg);
+      q.rows = int(M);
+      q.cols = int(K);
+      q.k_len = int(N);
+      q.c[0] = ptr(0);
+      product<DGRAD>(type, make_plan(DGRAD, M, K, N), q, opt);
+    }
+    if (need & 6) {
+      // one of the two alone: the other is computed beside it
+      at::Tensor spare;
+      if ((need & 6) != 6) spare = at::empty({K, N}, opt);
+      ProductArgs q{};
+      q.a[0] = q.a[1] = cptr(x);
+      q.b[0] = dg;
+      q.b[1] = du;
+      q.lda = ld_of(x);
+      q.ldb = ldg;
+      q.rows = int(K);
+      q.cols = int(N);
+      q.k_len = int(M);
+      q.c[0] = need & 2 ? ptr(1) : mptr(spare);
+      q.c[1] = need & 4 ? ptr(2) : mptr(spare);
+      product<WGRAD>(type, make_plan(WGRAD, K, N, M), q, opt);
+    }
+  }
+  for (int i = 0; i < 5; ++i)
+    if (result[i].defined() && result[i].scalar_type() != type)
+      result[i].view(-1).copy_(grads[i].view(-1));
+  return result;
+}
+
+}  // namespace dvgg

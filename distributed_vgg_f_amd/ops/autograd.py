@@ -102,6 +102,39 @@ class LinearFunction(torch.autograd.Function):
         return dx, _fresh(dw), _fresh(db), None
 
 
+class GatedLinearFunction(torch.autograd.Function):
+    """act(x w_gate + b_gate) * (x w_up + b_up) and its dropout. Keeps both
+    projections; backward is one pass over them and two products."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, act: int, p: float,
+                seed: int, offset):
+        on_device = isinstance(offset, torch.Tensor)
+        h, *saved = _ext().gated_fwd(
+            x, w_gate, w_up, bias_gate, bias_up, act, p, seed,
+            0 if on_device else offset, offset if on_device else None, True)
+        ctx.save_for_backward(*saved)
+        ctx.args = act, p, seed, 0 if on_device else offset
+        ctx.shape = w_gate.shape
+        # direct-grad: arena views attached by ArenaOptimizer
+        ctx.outs = [None] + [getattr(t, "_dvgg_gbuf", None)
+                             for t in (w_gate, w_up, bias_gate, bias_up)]
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        if torch.is_grad_enabled():     # the gradients' own graph is wanted
+            raise RuntimeError("gated_linear differentiates once: no "
+                               "create_graph=True through it")
+        gu, x, w_gate, w_up, *used = ctx.saved_tensors
+        need = sum(1 << i for i in range(5) if ctx.needs_input_grad[i])
+        grads = _ext().gated_bwd(dh, gu, x, w_gate, w_up, *ctx.shape,
+                                 *ctx.args, used[0] if used else None, need,
+                                 ctx.outs)
+        return (grads[0], *(_fresh(g) for g in grads[1:]),
+                None, None, None, None)
+
+
 class LRNFunction(torch.autograd.Function):
     """K4/K5. Fwd saves only x: backward recomputes the window scale s
     (cheap FMAs over the x it reloads anyway) and sb/snb via the same

@@ -69,6 +69,30 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     return y
 
 
+# the gated unit's activations, in the order of the kernels' numbers
+ACTIVATIONS = {
+    "silu": F.silu,
+    "gelu": F.gelu,
+    "gelu_tanh": lambda g: F.gelu(g, approximate="tanh"),
+    "relu": F.relu,
+    "sigmoid": torch.sigmoid,
+}
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                 bias_gate: Optional[torch.Tensor],
+                 bias_up: Optional[torch.Tensor],
+                 act: str = "silu") -> torch.Tensor:
+    """act(x @ w_gate + bias_gate) * (x @ w_up + bias_up); x [..., K],
+    w [K,N]."""
+    g, u = x @ w_gate, x @ w_up
+    if bias_gate is not None:
+        g = g + bias_gate
+    if bias_up is not None:
+        u = u + bias_up
+    return ACTIVATIONS[act](g) * u
+
+
 def dropout(x: torch.Tensor, p: float, mask: torch.Tensor) -> torch.Tensor:
     """Deterministic-mask dropout (mask supplied so CPU/GPU can be compared).
 
