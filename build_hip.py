@@ -21,7 +21,7 @@ OUT = os.path.join(ROOT, "distributed_vgg_f_amd", "_hipops.so")
 
 SOURCES = ["gemm_ops.hip", "mem.hip", "lrnpool.hip", "softbn.hip",
            "dropout.hip", "gated.hip",
-           "hipops.cpp"]
+           "fn.cpp", "hipops.cpp"]
 HEADERS = ["common.h", "gemm_tile.h", "gemm8.h", "wgrad_fused.h",
            "philox.h", "mfma_tile.h",
            "conv_ring.h"]

@@ -1,0 +1,140 @@
+// Autograd nodes of the operators in dropout.hip and gated.hip. In C++ because
+// the small calls are bound by what the host does: 256 x 4096 dropout forward
+// and backward took 31 us with nodes in Python for two kernels of 3 us.
+
+#include <torch/extension.h>
+
+namespace dvgg {
+
+std::vector<at::Tensor> dropout(const at::Tensor&, double, int64_t, int64_t,
+                                const c10::optional<at::Tensor>&);
+std::vector<at::Tensor> gated_fwd(
+    const at::Tensor&, const at::Tensor&, const at::Tensor&,
+    const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&,
+    int64_t, double, int64_t, int64_t, const c10::optional<at::Tensor>&,
+    bool);
+std::vector<at::Tensor> gated_bwd(
+    const at::Tensor&, const at::Tensor&, const at::Tensor&,
+    const at::Tensor&, const at::Tensor&, int64_t, int64_t, int64_t, double,
+    int64_t, int64_t, const c10::optional<at::Tensor>&, int64_t,
+    const std::vector<c10::optional<at::Tensor>>&);
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<at::Tensor>;
+
+// Backward draws the mask again from (p, seed, offset) and runs the forward's
+// kernel on dy. An offset from the device comes back from the kernel as the
+// value that it drew with: the caller may count the tensor up meanwhile.
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& x, double p,
+                          int64_t seed, int64_t offset,
+                          const OptTensor& offset_t) {
+    auto r = dropout(x.contiguous(), p, seed, offset, offset_t);
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["offset"] = offset;
+    if (r.size() > 1) ctx->save_for_backward({r[1]});
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    auto saved = ctx->get_saved_variables();
+    OptTensor used;
+    if (!saved.empty()) used = saved[0];
+    const double p = ctx->saved_data["p"].toDouble();
+    const int64_t seed = ctx->saved_data["seed"].toInt();
+    const int64_t offset = ctx->saved_data["offset"].toInt();
+    Variable dx;
+    if (grads[0].defined())
+      dx = at::GradMode::is_enabled()
+               ? DropoutFn::apply(grads[0], p, seed, offset, used)
+               : dropout(grads[0].contiguous(), p, seed, offset, used)[0];
+    return {dx, Variable(), Variable(), Variable(), Variable()};
+  }
+};
+
+at::Tensor dropout_ad(const at::Tensor& x, double p, int64_t seed,
+                      int64_t offset, const OptTensor& offset_t) {
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return DropoutFn::apply(x, p, seed, offset, offset_t);
+  return dropout(x.contiguous(), p, seed, offset, offset_t)[0];
+}
+
+// Keeps both projections; backward is one pass over them and two products.
+// *_out: gradient buffers of the engine's arena, written in place. What is
+// returned for them is a fresh view: AccumulateGrad stores a gradient only
+// if nothing else refers to its TensorImpl, and copies it otherwise.
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& x,
+                          const Variable& wg, const Variable& wu,
+                          const OptTensor& bg, const OptTensor& bu,
+                          int64_t act, double p, int64_t seed, int64_t offset,
+                          const OptTensor& offset_t,
+                          const std::vector<OptTensor>& outs) {
+    auto r = gated_fwd(x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
+                       true);
+    auto h = r[0];
+    r.erase(r.begin());
+    ctx->save_for_backward(r);
+    ctx->saved_data["K"] = wg.size(0);
+    ctx->saved_data["N"] = wg.size(1);
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["offset"] = offset;
+    // which of the five operands are there, in the order of gated_bwd
+    ctx->saved_data["bias"] = int64_t(bg.has_value()) | int64_t(
+        bu.has_value()) << 1;
+    for (int i = 0; i < 4; ++i)
+      if (outs[i]) ctx->saved_data[OUT[i]] = *outs[i];
+    return h;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "gated_linear differentiates "
+                "once: no create_graph=True through it");
+    auto& d = ctx->saved_data;
+    auto s = ctx->get_saved_variables();
+    const int64_t bias = d["bias"].toInt();
+    int64_t need = 0;
+    size_t edge = 0;              // only operands that are there have one
+    for (int i = 0; i < 5; ++i)
+      if ((i < 3 || bias >> (i - 3) & 1) && ctx->needs_input_grad(edge++))
+        need |= int64_t(1) << i;
+    variable_list result(11);
+    if (!grads[0].defined()) return result;
+    std::vector<OptTensor> outs(5);
+    for (int i = 0; i < 4; ++i) {
+      auto it = d.find(OUT[i]);
+      if (it != d.end()) outs[i + 1] = it->second.toTensor();
+    }
+    OptTensor used;
+    if (s.size() > 4) used = s[4];
+    auto r = gated_bwd(grads[0], s[0], s[1], s[2], s[3], d["K"].toInt(),
+                       d["N"].toInt(), d["act"].toInt(), d["p"].toDouble(),
+                       d["seed"].toInt(), d["offset"].toInt(), used, need,
+                       outs);
+    for (int i = 0; i < 5; ++i)
+      if (r[i].defined())
+        result[i] = outs[i] ? r[i].view(r[i].sizes()) : r[i];
+    return result;
+  }
+  static constexpr const char* OUT[4] = {"gate_out", "up_out", "bg_out",
+                                         "bu_out"};
+};
+
+at::Tensor gated_ad(const at::Tensor& x, const at::Tensor& wg,
+                    const at::Tensor& wu, const OptTensor& bg,
+                    const OptTensor& bu, int64_t act, double p, int64_t seed,
+                    int64_t offset, const OptTensor& offset_t,
+                    const std::vector<OptTensor>& outs) {
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || wg.requires_grad() || wu.requires_grad() ||
+       (bg && bg->requires_grad()) || (bu && bu->requires_grad())))
+    return GatedFn::apply(x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
+                          outs);
+  return gated_fwd(x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
+                   false)[0];
+}
+
+}  // namespace dvgg

@@ -12,9 +12,11 @@
 // one pass over dH, G and U, then two products on the same tiles.
 //
 // Roundings: sums, biases, the activation and the column sums stay in 32
-// bits. G and U are kept for the backward pass, and dG and dU handed to the
-// products, in the type of x: the matrix instructions take 16 bits, and 32
-// would double what the pass between them moves. Each is off by half a step.
+// bits, and so do G and U kept for the backward pass: rounded to 16 they
+// nearly double the error of the gradients (bf16, 256 x 9216 x 4096: 0.0031
+// of their size instead of 0.0024, one rounding of the result being 0.0017),
+// and they are 4 % of the time at the largest sizes, less elsewhere. dG and
+// dU are rounded to the type of x, which the matrix instructions take.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -32,7 +34,8 @@ DEV float to_f(u16 v, __bf16) { return bf2f(v); }
 DEV float to_f(u16 v, _Float16) {
   return float(__builtin_bit_cast(_Float16, v));
 }
-DEV u16 from_f(float v, __bf16) { return f2bf(v); }
+// one v_cvt_pk for two; round to nearest even, as f2bf
+DEV u16 from_f(float v, __bf16) { return __builtin_bit_cast(u16, __bf16(v)); }
 DEV u16 from_f(float v, _Float16) {
   return __builtin_bit_cast(u16, _Float16(v));
 }
@@ -40,50 +43,70 @@ DEV u16 from_f(float v, _Float16) {
 // ------------------------------------------------------------- activations
 enum Act { SILU, GELU, GELU_TANH, RELU, SIGMOID };
 
-DEV float sigmoid_f(float z) { return __frcp_rn(1.f + __expf(-z)); }
-
-// act(g) and act'(g). tanh(z) = 2 sigmoid(2z) - 1, so the tanh form of gelu
-// is g sigmoid(2z): nothing cancels. NaN passes through all of them.
-DEV float act_f(int act, float g, float& d) {
-  if (act == RELU) {
-    d = g <= 0.f ? 0.f : 1.f;
-    return g <= 0.f ? 0.f : g;
-  }
-  if (act == GELU) {
-    float c = 0.5f * erfcf(-0.70710678118654752f * g);
-    d = c + g * 0.39894228040143268f * __expf(-0.5f * g * g);
-    return g * c;
-  }
-  if (act == GELU_TANH) {
-    float z2 = 1.5957691216057308f * (g + 0.044715f * g * g * g);
-    float s = sigmoid_f(z2), w = s * (1.f - s);
-    // w is 0 where g * g no longer fits 32 bits
-    d = w > 0.f ? s + g * w * 1.5957691216057308f *
-                          (1.f + 0.134145f * g * g) : s;
-    return g * s;
-  }
-  float s = sigmoid_f(g);
-  if (act == SIGMOID) {
-    d = s * (1.f - s);
-    return s;
-  }
-  d = s * (1.f + g * (1.f - s));
-  return g * s;
+DEV float sigmoid_f(float z) {
+  return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
 
-// Bits 0..3: which of the 4 elements from flat index i stay. Their block of
-// the generator is one if i is a multiple of 4, else two.
-DEV u32 keep_from(const DropArgs& d, u32 off, i64 i) {
-  u32 sh = u32(i & 3);
-  u32 k = keep4(d, off, i >> 2);
-  if (sh) k = (k | keep4(d, off, (i >> 2) + 1) << 4) >> sh;
-  return k & 15u;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+
+// act(g) and act'(g) of 8 elements; the switch stands outside their loop.
+// tanh(z) = 2 sigmoid(2z) - 1, so the tanh form of gelu is g sigmoid(2z):
+// nothing cancels. NaN passes through all of them.
+template <class F>
+DEV f32x8 each(f32x8 g, F f) {
+#pragma unroll
+  for (int r = 0; r < 8; ++r) g[r] = f(g[r], r);
+  return g;
+}
+DEV f32x8 act8(int act, f32x8 g, f32x8& d) {
+  switch (act) {
+    case RELU:
+      d = each(g, [](float v, int) { return v <= 0.f ? 0.f : 1.f; });
+      return each(g, [](float v, int) { return v <= 0.f ? 0.f : v; });
+    case GELU:
+      return each(g, [&](float v, int r) {
+        float c = 0.5f * erfcf(-0.70710678118654752f * v);
+        d[r] = c + v * 0.39894228040143268f * __expf(-0.5f * v * v);
+        return v * c;
+      });
+    case GELU_TANH:
+      return each(g, [&](float v, int r) {
+        float s = sigmoid_f(1.5957691216057308f * (v + 0.044715f * v * v * v));
+        float w = s * (1.f - s);
+        // w is 0 where v * v no longer fits 32 bits
+        d[r] = w > 0.f ? s + v * w * 1.5957691216057308f *
+                             (1.f + 0.134145f * v * v) : s;
+        return v * s;
+      });
+    case SIGMOID:
+      return each(g, [&](float v, int r) {
+        float s = sigmoid_f(v);
+        d[r] = s * (1.f - s);
+        return s;
+      });
+    default:
+      return each(g, [&](float v, int r) {
+        float s = sigmoid_f(v);
+        d[r] = s * (1.f + v * (1.f - s));
+        return v * s;
+      });
+  }
+}
+
+// Bits 0..7: which of the 8 elements from flat index i stay. They lie in two
+// blocks of the generator if i is a multiple of 4, else in three.
+DEV u32 keep8(const DropArgs& d, u32 off, i64 i) {
+  const u32 sh = u32(i & 3);
+  i >>= 2;
+  u32 k = keep4(d, off, i) | keep4(d, off, i + 1) << 4;
+  if (sh) k = (k | keep4(d, off, i + 2) << 8) >> sh;
+  return k & 255u;
 }
 
 // ---------------------------------------------------------------- epilogue
 struct OutArgs {
   u16* h;             // [M][N]
-  u16* gu;            // [2][M][ldg] or null
+  float* gu;          // [2][M][ldg] or null
   const u16* bias[2]; // [N] or null
   int M, N;
   i64 ldg;
@@ -92,50 +115,69 @@ struct OutArgs {
   DropArgs d;
 };
 
-// Four columns of one row: g and u without their biases.
-template <class T>
-DEV void finish4(const OutArgs& o, u32 off, int m, int n, f32x4 g, f32x4 u) {
-  u32 keep = o.drop ? keep_from(o.d, off, (i64)m * o.N + n) : 15u;
-  s16x4 hv, gv, uv;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    int c = min(n + r, o.N - 1);
-    float gr = g[r], ur = u[r], d;
-    if (o.bias[0]) gr += to_f(o.bias[0][c], T());
-    if (o.bias[1]) ur += to_f(o.bias[1][c], T());
-    float h = act_f(o.act, gr, d) * ur;
-    if (o.drop) h = (keep >> r & 1) ? h * o.d.scale : 0.f;
-    hv[r] = short(from_f(h, T()));
-    gv[r] = short(from_f(gr, T()));
-    uv[r] = short(from_f(ur, T()));
-  }
-  u16* hp = o.h + (i64)m * o.N + n;
-  if ((o.N & 3) == 0) {
-    *reinterpret_cast<s16x4*>(hp) = hv;
+DEV f32x8 load8f(const float* v) {
+  f32x4 a = *reinterpret_cast<const f32x4*>(v);
+  f32x4 b = *reinterpret_cast<const f32x4*>(v + 4);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+DEV void store8f(float* p, f32x8 v) {
+  *reinterpret_cast<f32x4*>(p) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+  *reinterpret_cast<f32x4*>(p + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+}
+
+// 8 columns to row c of N
+DEV void store8(u16* c, int n, int N, s16x8 v) {
+  if ((N & 7) == 0) {
+    *reinterpret_cast<s16x8*>(c + n) = v;
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < o.N) hp[r] = u16(hv[r]);
-  }
-  if (o.gu) {         // rows of ldg, a multiple of 8, hold all four
-    u16* gp = o.gu + (i64)m * o.ldg + n;
-    *reinterpret_cast<s16x4*>(gp) = gv;
-    *reinterpret_cast<s16x4*>(gp + (i64)o.M * o.ldg) = uv;
+    for (int r = 0; r < 8; ++r)
+      if (n + r < N) c[n + r] = u16(v[r]);
   }
 }
 
 template <class T>
-DEV void store4(u16* c, int n, int N, f32x4 v) {
-  s16x4 o;
+DEV s16x8 round8(f32x8 v) {
+  s16x8 o;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) o[r] = short(from_f(v[r], T()));
-  if ((N & 3) == 0) {
-    *reinterpret_cast<s16x4*>(c + n) = o;
-  } else {
+  for (int r = 0; r < 8; ++r) o[r] = short(from_f(v[r], T()));
+  return o;
+}
+
+template <class T>
+DEV f32x8 widen8(s16x8 v) {
+  f32x8 o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < N) c[n + r] = u16(o[r]);
+  for (int r = 0; r < 8; ++r) o[r] = to_f(u16(v[r]), T());
+  return o;
+}
+
+// 8 columns of one row, n a multiple of 8: g and u without their biases.
+template <class T>
+DEV void finish8(const OutArgs& o, u32 off, int m, int n, f32x8 g, f32x8 u) {
+  if (o.bias[0]) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      g[r] += to_f(o.bias[0][min(n + r, o.N - 1)], T());
   }
+  if (o.bias[1]) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      u[r] += to_f(o.bias[1][min(n + r, o.N - 1)], T());
+  }
+  if (o.gu) {         // rows of ldg, a multiple of 8, hold all eight
+    float* gp = o.gu + (i64)m * o.ldg + n;
+    store8f(gp, g);
+    store8f(gp + (i64)o.M * o.ldg, u);
+  }
+  f32x8 d;
+  u *= act8(o.act, g, d);
+  if (o.drop) {
+    const u32 keep = keep8(o.d, off, (i64)m * o.N + n);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) u[r] = (keep >> r & 1) ? u[r] * o.d.scale : 0.f;
+  }
+  store8(o.h + (i64)m * o.N, n, o.N, round8<T>(u));
 }
 
 // ---------------------------------------------------------------- products
@@ -152,45 +194,48 @@ struct ProductArgs {
   int k_len;
   int splits, stages;   // stages of one part of the contraction
   int tiles_m, tiles_n;
-  float* slab;          // [splits][2 or 1][rows][cols4] if splits > 1
-  i64 slab_ld;          // cols rounded up to 4
+  float* slab;          // [splits][2 or 1][rows][slab_ld] if splits > 1
+  i64 slab_ld;          // cols rounded up to 8
   u16* c[2];            // outputs of DGRAD ([0]) and WGRAD
   OutArgs out;          // of FWD
 };
 
-// Four columns of each half of a tile's row.
+// Eight columns of a row of DGRAD or WGRAD.
 template <class T, int MODE>
-DEV void emit(const ProductArgs& p, int split, int which, u32 off, int m,
-              int n, int n2, f32x4 v0, f32x4 v1) {
-  if (MODE == FWD) {
-    if (n >= p.cols) return;
-    if (p.splits == 1) {
-      finish4<T>(p.out, off, m, n, v0, v1);
-    } else {
-      float* sp = p.slab + ((i64)split * 2 * p.rows + m) * p.slab_ld + n;
-      *reinterpret_cast<f32x4*>(sp) = v0;
-      *reinterpret_cast<f32x4*>(sp + (i64)p.rows * p.slab_ld) = v1;
-    }
-  } else if (p.splits == 1) {
-    u16* c = (which ? p.c[1] : p.c[0]) + (i64)m * p.cols;
-    if (n < p.cols) store4<T>(c, n, p.cols, v0);
-    if (n2 < p.cols) store4<T>(c, n2, p.cols, v1);
+DEV void emit(const ProductArgs& p, int split, int which, int m, int n,
+              f32x8 v) {
+  if (n >= p.cols) return;
+  if (p.splits == 1) {
+    store8((which ? p.c[1] : p.c[0]) + (i64)m * p.cols, n, p.cols,
+           round8<T>(v));
   } else {
     constexpr int MATS = MODE == WGRAD ? 2 : 1;
-    float* sp = p.slab +
-        (((i64)split * MATS + which) * p.rows + m) * p.slab_ld;
-    if (n < p.cols) *reinterpret_cast<f32x4*>(sp + n) = v0;
-    if (n2 < p.cols) *reinterpret_cast<f32x4*>(sp + n2) = v1;
+    store8f(p.slab + (((i64)split * MATS + which) * p.rows + m) * p.slab_ld +
+                n, v);
+  }
+}
+// Eight columns of G and U.
+template <class T>
+DEV void emit_gated(const ProductArgs& p, int split, u32 off, int m, int n,
+                    f32x8 g, f32x8 u) {
+  if (n >= p.cols) return;
+  if (p.splits == 1) {
+    finish8<T>(p.out, off, m, n, g, u);
+  } else {
+    float* sp = p.slab + ((i64)split * 2 * p.rows + m) * p.slab_ld + n;
+    store8f(sp, g);
+    store8f(sp + (i64)p.rows * p.slab_ld, u);
   }
 }
 
-template <class T, int MODE, int FM, int FN>
+template <class T, int MODE, int FM, int FN, bool SHORT = false>
 __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
   constexpr bool ATR = MODE == WGRAD, BTR = MODE != DGRAD;
-  using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN>;
+  using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN, MODE == FWD,
+                  SHORT>;
   // two objects, so that reads of one do not wait for loads into the other
   __shared__ __attribute__((aligned(1024))) char even[TL::STAGE];
-  __shared__ __attribute__((aligned(1024))) char odd[TL::STAGE];
+  __shared__ __attribute__((aligned(1024))) char odd[SHORT ? 16 : TL::STAGE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -237,59 +282,71 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
   TL tile;
   tile.run((lds_char*)even, (lds_char*)odd, s, wave, lane, acc);
 
-  // Through LDS, 32 rows of a wave at a time: the lanes then hold whole
-  // stretches of 64 columns of a row (128 bytes a store), and one copy of the
-  // epilogue's code per 32 rows is enough.
+  // Through LDS, some rows of a wave at a time: the lanes then hold whole
+  // stretches of a row (128 bytes a store and more), and one copy of the
+  // epilogue's code for these rows is enough.
+  constexpr int ROWS = SHORT ? 16 : 32;
   constexpr int PITCH = 16 * FN + 4;      // floats; + 4: rows change banks
-  static_assert(32 * PITCH * 4 <= TL::STAGE / 2, "a wave's part of a stage");
+  constexpr int MINE = SHORT ? TL::STAGE / 4 : TL::STAGE / 2;
+  static_assert(ROWS * PITCH * 4 <= MINE, "a wave's part of the LDS");
   float* mine = reinterpret_cast<float*>(
-      (wave & 2 ? odd : even) + (wave & 1) * (TL::STAGE / 2));
+      SHORT ? even + wave * MINE
+            : (wave & 2 ? odd : even) + (wave & 1) * MINE);
   __syncthreads();
   const u32 off = MODE == FWD && p.out.drop ? p.out.d.off() : 0;
-  const int nw = n0 + (wave & 1) * 8 * FN;
 #pragma unroll
-  for (int i = 0; i < FM; i += 2) {
+  for (int i = 0; i < FM; i += ROWS / 16) {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+      for (int q = 0; q < ROWS / 16; ++q)
         *reinterpret_cast<f32x4*>(mine + (q * 16 + (lane & 15)) * PITCH +
                                   j * 16 + (lane >> 4) * 4) = acc[i + q][j];
     // one wave writes and reads: its LDS instructions keep their order
     const int mw = m0 + (wave >> 1) * 16 * FM + i * 16;
-    constexpr int CH = 2 * FN;            // 4-column chunks of a half row
+    if (MODE == FWD) {
+      const int nw = n0 + (wave & 1) * 8 * FN;
 #pragma unroll 1
-    for (int c = lane; c < 32 * CH; c += 64) {
-      const int m = mw + c / CH, n = nw + c % CH * 4;
-      const float* v = mine + c / CH * PITCH + c % CH * 4;
-      f32x4 v0 = *reinterpret_cast<const f32x4*>(v);
-      f32x4 v1 = *reinterpret_cast<const f32x4*>(v + 8 * FN);
-      if (m >= p.rows) break;
-      emit<T, MODE>(p, split, which, off, m, n, n + TL::HALF, v0, v1);
+      for (int c = lane; c < ROWS * FN; c += 64) {
+        const int m = mw + c / FN, n = c % FN * 8;
+        const float* v = mine + c / FN * PITCH + n;
+        if (m >= p.rows) break;
+        emit_gated<T>(p, split, off, m, nw + n, load8f(v),
+                      load8f(v + 8 * FN));
+      }
+    } else {
+      const int nw = n0 + (wave & 1) * TL::HALF;
+#pragma unroll 2
+      for (int c = lane; c < ROWS * 2 * FN; c += 64) {
+        const int m = mw + c / (2 * FN), n = c % (2 * FN) * 8;
+        f32x8 v = load8f(mine + c / (2 * FN) * PITCH + n);
+        if (m < p.rows) emit<T, MODE>(p, split, which, m, nw + n, v);
+      }
     }
   }
 }
 
 // ------------------------------------------------- joining a split product
-// Sums the slabs in their order (the same result every time), 4 columns a
+// Sums the slabs in their order (the same result every time), 8 columns a
 // thread.
 template <class T>
 __global__ __launch_bounds__(256) void join_gated_kernel(
     const float* __restrict__ slab, int splits, i64 slab_ld, OutArgs o) {
   const u32 off = o.drop ? o.d.off() : 0;
-  const int cols4 = int(slab_ld / 4);
+  const int per = int(slab_ld / 8);
   const i64 one = (i64)o.M * slab_ld;
-  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < (i64)o.M * cols4;
+  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < (i64)o.M * per;
        c += (i64)gridDim.x * 256) {
-    const float* sp = slab + c * 4;
-    f32x4 g{0.f, 0.f, 0.f, 0.f}, u = g;
+    const float* sp = slab + c * 8;
+    f32x8 g{}, u{};
+#pragma unroll 2
     for (int s = 0; s < splits; ++s) {
-      g += *reinterpret_cast<const f32x4*>(sp);
-      u += *reinterpret_cast<const f32x4*>(sp + one);
+      g += load8f(sp);
+      u += load8f(sp + one);
       sp += 2 * one;
     }
-    int m = int(c / cols4);
-    finish4<T>(o, off, m, int(c - (i64)m * cols4) * 4, g, u);
+    int m = int(c / per);
+    finish8<T>(o, off, m, int(c - (i64)m * per) * 8, g, u);
   }
 }
 
@@ -297,18 +354,18 @@ template <class T>
 __global__ __launch_bounds__(256) void join_plain_kernel(
     const float* __restrict__ slab, int splits, i64 slab_ld, int rows,
     int cols, int mats, u16* c0, u16* c1) {
-  const int cols4 = int(slab_ld / 4);
+  const int per = int(slab_ld / 8);
   const i64 one = (i64)rows * slab_ld * mats;
   for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x;
-       c < (i64)rows * mats * cols4; c += (i64)gridDim.x * 256) {
-    const float* sp = slab + c * 4;
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s, sp += one)
-      v += *reinterpret_cast<const f32x4*>(sp);
-    i64 m = c / cols4;
-    int n = int(c - m * cols4) * 4;
+       c < (i64)rows * mats * per; c += (i64)gridDim.x * 256) {
+    const float* sp = slab + c * 8;
+    f32x8 v{};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s, sp += one) v += load8f(sp);
+    i64 m = c / per;
+    int n = int(c - m * per) * 8;
     u16* out = m < rows ? c0 + m * cols : c1 + (m - rows) * cols;
-    store4<T>(out, n, cols, v);
+    store8(out, n, cols, round8<T>(v));
   }
 }
 
@@ -319,7 +376,7 @@ __global__ __launch_bounds__(256) void join_plain_kernel(
 struct MidArgs {
   const u16* dh;
   i64 ldh;
-  const u16* gu;
+  const float* gu;
   u16* dgu;
   float* part;
   int M, N;
@@ -335,16 +392,15 @@ __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int n = blockIdx.x * 256 + tx * 8;
   const u32 off = a.drop ? a.d.off() : 0;
-  float sg[8] = {}, su[8] = {};
+  f32x8 sg{}, su{};
   const int r0 = blockIdx.y * a.rows_per_block;
   const int r1 = min(a.M, r0 + a.rows_per_block);
   const bool wide = (a.N & 7) == 0 && (a.ldh & 7) == 0 &&
                     (reinterpret_cast<uintptr_t>(a.dh) & 15) == 0;
   if (n < a.ldg) {
     for (int m = r0 + ty; m < r1; m += 8) {
-      const u16* gp = a.gu + (i64)m * a.ldg + n;
-      s16x8 g = *reinterpret_cast<const s16x8*>(gp);
-      s16x8 u = *reinterpret_cast<const s16x8*>(gp + (i64)a.M * a.ldg);
+      const float* gp = a.gu + (i64)m * a.ldg + n;
+      f32x8 g = load8f(gp), u = load8f(gp + (i64)a.M * a.ldg);
       s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
       const u16* hp = a.dh + (i64)m * a.ldh + n;
       if (wide) {
@@ -357,22 +413,20 @@ __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
       u32 keep = 255u;
       if (a.drop) {
         i64 i = (i64)m * a.N + n;
-        keep = keep_from(a.d, off, i) | keep_from(a.d, off, i + 4) << 4;
+        keep = keep8(a.d, off, i);
       }
-      s16x8 og, ou;
+      f32x8 d, act = act8(a.act, g, d), v = widen8<T>(h), dg, du;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float d, v = to_f(u16(h[j]), T());
-        float act = act_f(a.act, to_f(u16(g[j]), T()), d);
-        if (a.drop) v *= a.d.scale;
-        float dg = v * to_f(u16(u[j]), T()) * d, du = v * act;
+        if (a.drop) v[j] *= a.d.scale;
         // what was dropped, or lies behind N, passes nothing on
-        if (!(keep >> j & 1) || n + j >= a.N) dg = du = 0.f;
-        sg[j] += dg;
-        su[j] += du;
-        og[j] = short(from_f(dg, T()));
-        ou[j] = short(from_f(du, T()));
+        const bool in = (keep >> j & 1) && n + j < a.N;
+        dg[j] = in ? v[j] * u[j] * d[j] : 0.f;
+        du[j] = in ? v[j] * act[j] : 0.f;
       }
+      sg += dg;
+      su += du;
+      s16x8 og = round8<T>(dg), ou = round8<T>(du);
       u16* op = a.dgu + (i64)m * a.ldg + n;
       *reinterpret_cast<s16x8*>(op) = og;
       *reinterpret_cast<s16x8*>(op + (i64)a.M * a.ldg) = ou;
@@ -398,17 +452,27 @@ __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
   pp[a.ldg] = vu;
 }
 
+// 32 columns a block, 8 groups of threads a part of the blocks' sums each.
 template <class T>
 __global__ __launch_bounds__(256) void bias_join_kernel(
     const float* __restrict__ part, int blocks, int N, i64 ldg, u16* dbg,
     u16* dbu) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= N) return;
+  __shared__ float red[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
   u16* out = blockIdx.y ? dbu : dbg;
   if (!out) return;
-  part += blockIdx.y * ldg + c;
   float v = 0.f;
-  for (int b = 0; b < blocks; ++b) v += part[(i64)b * 2 * ldg];
+  if (c < N) {
+    part += blockIdx.y * ldg + c;
+#pragma unroll 4
+    for (int b = ty; b < blocks; b += 8) v += part[(i64)b * 2 * ldg];
+  }
+  red[ty][tx] = v;
+  __syncthreads();
+  if (ty || c >= N) return;
+#pragma unroll
+  for (int r = 1; r < 8; ++r) v += red[r][tx];
   out[c] = from_f(v, T());
 }
 
@@ -464,37 +528,78 @@ static i64 ld_of(const at::Tensor& t) {
   return t.size(0) == 1 ? t.size(1) : t.stride(0);
 }
 
-struct Plan { int fm, fn, splits, tiles_m, tiles_n, stages; };
+struct Plan { int fm, fn, splits, tiles_m, tiles_n, stages; bool brief; };
 
+// Which tile, and into how many parts the contraction is split: the least
+// time by a model of what the tiles measured over 44 products from 1 x 512 to
+// 8192 x 8192 rows and columns (it is off by 13 % there; what it picks is 2 %
+// slower than the best of all tiles and splits in the mean, 17 % at worst).
+// Microseconds. A stage costs `one` if a tile has its CU to itself and `all`
+// if the CU is full; `edge` is a tile's first loads and its epilogue.
 static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
-  Plan p;
-  p.fm = rows > 128 ? 8 : rows > 64 ? 4 : 2;
-  p.fn = 8;
-  p.stages = ceil_div(k_len, TILE_BK);
-  p.tiles_m = ceil_div(rows, 32 * p.fm);
-  p.tiles_n = ceil_div(cols, mode == FWD ? 16 * p.fn : 32 * p.fn) *
-              (mode == WGRAD ? 2 : 1);
-  i64 tiles = (i64)p.tiles_m * p.tiles_n;
-  p.splits = 1;
-  while (tiles * p.splits * 2 <= 256 && p.stages / (p.splits * 2) >= 8)
-    p.splits *= 2;
-  return p;
+  struct Kind { int fm, fn, per_cu; double one, all, edge; bool brief; };
+  static const Kind kinds[] = {{8, 8, 1, 1.24, 1.24, 9.8, false},
+                               {4, 4, 2, 0.69, 0.96, 3.9, false},
+                               {2, 4, 3, 0.61, 0.93, 2.8, false},
+                               {4, 4, 3, 0.69, 0.96, 3.9, true}};
+  constexpr double CUS = 256, MEM = 4.5e6, JOIN = 2.8, JOIN_MEM = 7e6;
+  const int stages = ceil_div(k_len, TILE_BK);
+  const double mats = mode == DGRAD ? 1 : 2, parts = mode == DGRAD ? 2 : 1;
+  const double out = double(rows) * cols;
+  // bytes that the product moves at least
+  const double ab = mode == FWD ? rows + 2. * cols
+                  : mode == DGRAD ? 2. * rows + 2. * cols : rows + 2. * cols;
+  const double mem = 2 * (ab * k_len + (mode == FWD ? 3 : mats) * out) / MEM;
+  Plan best{};
+  double least = 0;
+  for (const Kind& k : kinds) {
+    if (k.brief && (mode != WGRAD || stages > 1)) continue;
+    const int tm = ceil_div(rows, 32 * k.fm);
+    const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
+                   (mode == WGRAD ? 2 : 1);
+    for (int sp = 1; sp <= stages && sp <= 32; sp += sp < 4 ? 1 : sp / 2) {
+      const double wgs = double(tm) * tn * sp, slots = CUS * k.per_cu;
+      const double depth = ceil_div(stages, sp) * parts;
+      auto round = [&](double n) {
+        const double share = k.per_cu > 1
+            ? (std::ceil(n / CUS) - 1) / (k.per_cu - 1) : 1;
+        return n > 0 ? k.edge + depth * (k.one + (k.all - k.one) * share) : 0;
+      };
+      const double full = std::floor(wgs / slots);
+      double t = full * round(slots) + round(wgs - full * slots);
+      t = std::sqrt(std::sqrt(t * t * t * t + mem * mem * mem * mem));
+      if (sp > 1) t += JOIN + sp * mats * out * 8 / JOIN_MEM;
+      if (least == 0 || t < least) {
+        least = t;
+        best = Plan{k.fm, k.fn, sp, tm, tn, stages, k.brief};
+      }
+    }
+  }
+  return best;
 }
 
 template <class T, int MODE>
 static void launch(const Plan& pl, const ProductArgs& a) {
   dim3 grid(u32(pl.tiles_m) * pl.tiles_n * pl.splits);
   auto st = cur_stream();
-  if (pl.fm == 8)
-    hipLaunchKernelGGL((product_kernel<T, MODE, 8, 8>), grid, dim3(256), 0,
-                       st, a);
-  else if (pl.fm == 4)
-    hipLaunchKernelGGL((product_kernel<T, MODE, 4, 8>), grid, dim3(256), 0,
-                       st, a);
-  else
-    hipLaunchKernelGGL((product_kernel<T, MODE, 2, 8>), grid, dim3(256), 0,
-                       st, a);
-  HIP_CHECK(hipGetLastError());
+  if (pl.brief) {
+    hipLaunchKernelGGL((product_kernel<T, WGRAD, 4, 4, true>), grid,
+                       dim3(256), 0, st, a);
+    HIP_CHECK(hipGetLastError());
+    return;
+  }
+#define TILE_CASE(FM, FN)                                                  \
+  if (pl.fm == FM && pl.fn == FN) {                                        \
+    hipLaunchKernelGGL((product_kernel<T, MODE, FM, FN>), grid, dim3(256), \
+                       0, st, a);                                          \
+    HIP_CHECK(hipGetLastError());                                          \
+    return;                                                                \
+  }
+  TILE_CASE(8, 8)
+  TILE_CASE(4, 4)
+  TILE_CASE(2, 4)
+#undef TILE_CASE
+  TORCH_CHECK(false, "gated_linear: no tile of this size");
 }
 
 template <int MODE>
@@ -504,7 +609,7 @@ static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
   a.stages = pl.stages;
   a.tiles_m = pl.tiles_m;
   a.tiles_n = pl.tiles_n;
-  a.slab_ld = up(a.cols, 4);
+  a.slab_ld = up(a.cols, 8);
   const int mats = MODE == DGRAD ? 1 : 2;
   at::Tensor slab;
   if (pl.splits > 1) {
@@ -516,7 +621,7 @@ static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
   if (half) launch<_Float16, MODE>(pl, a);
   else launch<__bf16, MODE>(pl, a);
   if (pl.splits == 1) return;
-  i64 chunks = (i64)a.rows * (MODE == WGRAD ? 2 : 1) * a.slab_ld / 4;
+  i64 chunks = (i64)a.rows * (MODE == WGRAD ? 2 : 1) * a.slab_ld / 8;
   dim3 grid(u32(std::min<i64>((chunks + 255) / 256, 8192)));
   auto st = cur_stream();
   if (MODE == FWD) {
@@ -570,7 +675,7 @@ static DropArgs gated_drop(const at::Tensor& x, double p, int64_t seed,
 __global__ void copy_offset_kernel(const i64* in, i64* out) { *out = *in; }
 
 // Returns h [M][N], and with `train` also what backward wants: G and U as
-// one [2][M][N up to a vector], the three operands as the tiles load them,
+// one [2][M][N up to a vector] in 32 bits, the three operands as the tiles load them,
 // and the offset that the mask was drawn with if it came from the device.
 std::vector<at::Tensor> gated_fwd(
     const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
@@ -599,7 +704,7 @@ std::vector<at::Tensor> gated_fwd(
   auto h = at::empty({M, N}, x.options());
   at::Tensor gu, used;
   const i64 ldg = up(N, 8);
-  if (train) gu = at::empty({2, M, ldg}, x.options());
+  if (train) gu = at::empty({2, M, ldg}, x.options().dtype(at::kFloat));
   if (train && offset_t) {
     used = at::empty({1}, offset_t->options());
     hipLaunchKernelGGL(copy_offset_kernel, dim3(1), dim3(1), 0, cur_stream(),
@@ -627,7 +732,7 @@ std::vector<at::Tensor> gated_fwd(
     a.rows = int(M);
     a.cols = int(N);
     a.k_len = int(K);
-    a.out = OutArgs{mptr(h), train ? mptr(gu) : nullptr,
+    a.out = OutArgs{mptr(h), train ? gu.data_ptr<float>() : nullptr,
                     {bg ? cptr(bgc) : nullptr, bu ? cptr(buc) : nullptr},
                     int(M), int(N), ldg, int(act), p > 0.0, d};
     product<FWD>(type, make_plan(FWD, M, N, K), a, x.options());
@@ -674,12 +779,12 @@ std::vector<at::Tensor> gated_bwd(
   if (M == 0) {
     for (auto& g : grads) if (g.defined()) g.zero_();
   } else {
-    auto dgu = at::empty_like(gu);
+    auto dgu = at::empty({2, M, ldg}, opt);
     const bool bias = (need & 24) != 0;
     MidArgs a{};
     a.dh = cptr(dh);
     a.ldh = M == 1 ? N : dh.stride(0);
-    a.gu = cptr(gu);
+    a.gu = gu.data_ptr<float>();
     a.dgu = mptr(dgu);
     a.M = int(M);
     a.N = int(N);
@@ -706,7 +811,7 @@ std::vector<at::Tensor> gated_bwd(
       hipLaunchKernelGGL(mid_kernel<__bf16>, dim3(bx, by), dim3(256), 0, st,
                          a);
     if (bias) {
-      dim3 g(ceil_div(N, 256), 2);
+      dim3 g(ceil_div(N, 32), 2);
       if (half)
         hipLaunchKernelGGL(bias_join_kernel<_Float16>, g, dim3(256), 0, st,
                            a.part, by, int(N), ldg, ptr(3), ptr(4));

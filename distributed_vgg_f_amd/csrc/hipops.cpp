@@ -35,21 +35,14 @@ std::vector<at::Tensor> dropout_fwd(const at::Tensor&, double, int64_t,
                                     int64_t);
 at::Tensor dropout_bwd(const at::Tensor&, const at::Tensor&, double);
 
-// dropout.hip
-std::vector<at::Tensor> dropout(const at::Tensor&, double, int64_t, int64_t,
-                                const c10::optional<at::Tensor>&);
-
-// gated.hip
-std::vector<at::Tensor> gated_fwd(
-    const at::Tensor&, const at::Tensor&, const at::Tensor&,
-    const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&,
-    int64_t, double, int64_t, int64_t, const c10::optional<at::Tensor>&,
-    bool);
-std::vector<at::Tensor> gated_bwd(
-    const at::Tensor&, const at::Tensor&, const at::Tensor&,
-    const at::Tensor&, const at::Tensor&, int64_t, int64_t, int64_t, double,
-    int64_t, int64_t, const c10::optional<at::Tensor>&, int64_t,
-    const std::vector<c10::optional<at::Tensor>>&);
+// fn.cpp
+at::Tensor dropout_ad(const at::Tensor&, double, int64_t, int64_t,
+                      const c10::optional<at::Tensor>&);
+at::Tensor gated_ad(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                    const c10::optional<at::Tensor>&,
+                    const c10::optional<at::Tensor>&, int64_t, double,
+                    int64_t, int64_t, const c10::optional<at::Tensor>&,
+                    const std::vector<c10::optional<at::Tensor>>&);
 
 // lrnpool.hip
 at::Tensor lrn_fwd(const at::Tensor&, int64_t, double, double, double);
@@ -102,14 +95,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bump_weight_gen", &dvgg::bump_weight_gen);
   m.def("dropout_fwd", &dvgg::dropout_fwd);
   m.def("dropout_bwd", &dvgg::dropout_bwd);
-  m.def("dropout", &dvgg::dropout, py::arg("x"), py::arg("p"),
+  m.def("dropout", &dvgg::dropout_ad, py::arg("x"), py::arg("p"),
         py::arg("seed"), py::arg("offset"),
         py::arg("offset_t") = c10::nullopt);
-  m.def("gated_fwd", &dvgg::gated_fwd, py::arg("x"), py::arg("w_gate"),
+  m.def("gated_linear", &dvgg::gated_ad, py::arg("x"), py::arg("w_gate"),
         py::arg("w_up"), py::arg("bias_gate"), py::arg("bias_up"),
         py::arg("act"), py::arg("p"), py::arg("seed"), py::arg("offset"),
-        py::arg("offset_t") = c10::nullopt, py::arg("train") = false);
-  m.def("gated_bwd", &dvgg::gated_bwd);
+        py::arg("offset_t"), py::arg("grad_outs"));
   m.def("lrn_fwd", &dvgg::lrn_fwd);
   m.def("lrn_bwd", &dvgg::lrn_bwd);
   m.def("maxpool_fwd", &dvgg::maxpool_fwd);

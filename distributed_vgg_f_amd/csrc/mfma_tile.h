@@ -164,18 +164,23 @@ struct TileSrc {
   int k_first, k_last;      // the contraction [k_first, k_last) of each part
 };
 
-template <class T, bool ATR, bool BTR, int PARTS, int FM, int FN>
+// PAIRED: a wave takes the same columns of both halves, else all columns of
+// one. SHORT: the whole contraction is one stage, which then is all the LDS
+// that the tile needs; more tiles share a CU.
+template <class T, bool ATR, bool BTR, int PARTS, int FM, int FN, bool PAIRED,
+          bool SHORT>
 struct Tile {
   static constexpr int BM = 32 * FM, BN = 32 * FN, HALF = BN / 2;
   using PA = Panel<ATR, BM>;
   using PB = Panel<BTR, HALF>;
   static constexpr int STAGE = PA::BYTES + 2 * PB::BYTES;
   static constexpr int LOADS = PA::LOADS + 2 * PB::LOADS;
+  static constexpr int FH = PAIRED ? FN / 2 : FN;  // fragments in a half
 
   PA pa;
   PB pb[2];
   Frags<ATR, BM, FM> ra;
-  Frags<BTR, HALF, FN / 2> rb;
+  Frags<BTR, HALF, FH> rb;
   s16x8 fa[FM], fb[FN];
   int wave;
 
@@ -198,35 +203,48 @@ struct Tile {
     fa[i] = ra.read(src, i, half);
   }
   DEV void fetch_b(const lds_char* src, int half, int j) {
-    fb[j] = rb.read(src + PA::BYTES + j / (FN / 2) * PB::BYTES, j % (FN / 2),
-                    half);
+    const int h = PAIRED ? j / FH : wave & 1;
+    fb[j] = rb.read(src + PA::BYTES + h * PB::BYTES, j % FH, half);
   }
 
-  // 32 k: the products of the fragments at hand, row by row of A, and behind
-  // the last use of each fragment the read of its successor, from half
-  // `half` of `src`. REFILL: the half that changes over to the next stage.
-  // After its first row every wave is done reading `dst` and its own loads
-  // into `src` have landed, so it syncs there, with products still queued,
-  // and spreads the loads that refill `dst` over the other rows.
-  template <bool REFILL, int PART>
-  DEV void step(const TileSrc& s, const lds_char* src, int half,
-                lds_char* dst, int k, f32x4 (&acc)[FM][FN]) {
+  // 32 k: the products of the fragments at hand, row by row of A. Between
+  // them, one or two at a time (a product keeps the matrix core for 16 cycles
+  // and issues in 4: bunched up, the others would hold it up):
+  //   - the read of each fragment's successor behind its last use, from half
+  //     `half` of `src` (LAST: there is none). That of A's last row comes in
+  //     the next step, so this one begins with its own, from `cur`;
+  //   - REFILL, the half that changes over to the next stage: after its first
+  //     rows every wave is done reading `dst` and its own loads into `src`
+  //     have landed, so it syncs there, with products still queued; then the
+  //     loads that refill `dst`.
+  enum Kind { PLAIN, REFILL, LAST };
+  template <Kind KIND, int PART>
+  DEV void step(const TileSrc& s, const lds_char* cur, const lds_char* src,
+                int half, lds_char* dst, int k, f32x4 (&acc)[FM][FN]) {
+    constexpr bool FILL = KIND == REFILL;
+    constexpr int ROW0 = !FILL ? 0 : FM > 2 ? 2 : 1;    // first row of reads
+    constexpr int SLOTS = (FM > 2 ? FM - 1 - ROW0 : 1) * FN;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         mfma32<T>(acc[i][j], fb[j], fa[i]);
-        if (i == FM - 1 && FM > 1) fetch_b(src, half, j);
-      }
-      if (i == 0 && REFILL) sync();
-      fetch_a(src, half, i);
-      if (REFILL) {
+        if (i == 0 && j == 1) fetch_a(cur, half ^ 1, FM - 1);
+        if (KIND != LAST && i >= ROW0) {
+          if (j == 1 && i > 0) fetch_a(src, half, i - 1);
+          if (j == 3 && i == 2 && ROW0 == 2) fetch_a(src, half, 0);
+          if (i == FM - 1) fetch_b(src, half, j);
+          if (FILL) {
+            const int t = (i - ROW0) * FN + j;
 #pragma unroll
-        for (int l = i * LOADS / FM; l < (i + 1) * LOADS / FM; ++l)
-          load<PART>(s, dst, k, l);
+            for (int l = 0; l < LOADS; ++l)
+              if (l * SLOTS / LOADS == t) load<PART>(s, dst, k, l);
+          }
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (FILL && i == ROW0 - 1) sync();
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // this wave's loads have landed and its reads are done; then all waves'
@@ -238,8 +256,9 @@ struct Tile {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // acc[i][j]: rows 16 i + lane % 16 of the wave's 16 FM, columns
-  // 16 (j % (FN/2)) + 4 (lane / 16) + 0..3 of its 8 FN in half j / (FN/2).
+  // acc[i][j]: rows 16 i + lane % 16 of the wave's 16 FM; columns
+  // 16 (j % FH) + 4 (lane / 16) + 0..3 of the wave's in half j / FH (PAIRED)
+  // or in its own half.
   DEV void run(lds_char* even, lds_char* odd, const TileSrc& s, int wave_,
                int lane, f32x4 (&acc)[FM][FN]) {
     constexpr int P1 = PARTS - 1;
@@ -250,25 +269,35 @@ struct Tile {
     pb[0].init(wave, lane, s.ldb, s.rows_b[0]);
     pb[1].init(wave, lane, s.ldb, s.rows_b[1]);
     ra.init(lane, (wave >> 1) * 16 * FM);
-    rb.init(lane, (wave & 1) * 8 * FN);
+    rb.init(lane, PAIRED ? (wave & 1) * 8 * FN : 0);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) load<0>(s, even, s.k_first, l);
+    if (!SHORT) {
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) load<P1>(s, odd, s.k_first + KODD, l);
+      for (int l = 0; l < LOADS; ++l) load<P1>(s, odd, s.k_first + KODD, l);
+    }
     sync();
 #pragma unroll
     for (int j = 0; j < FN; ++j) fetch_b(even, 0, j);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) fetch_a(even, 0, i);
-    for (int k = s.k_first; k < s.k_last; k += KTURN) {
-      step<false, 0>(s, even, 1, even, 0, acc);
-      step<true, 0>(s, odd, 0, even, k + KTURN, acc);
-      step<false, 0>(s, odd, 1, odd, 0, acc);
-      step<true, P1>(s, even, 0, odd, k + KTURN + KODD, acc);
+    for (int i = 0; i < FM - 1; ++i) fetch_a(even, 0, i);
+    int k = s.k_first;
+    if (!SHORT) {
+      // whole turns; a last single stage of one part is left for below
+      for (; k < s.k_last - KODD; k += KTURN) {
+        step<PLAIN, 0>(s, even, even, 1, even, 0, acc);
+        step<REFILL, 0>(s, even, odd, 0, even, k + KTURN, acc);
+        step<PLAIN, 0>(s, odd, odd, 1, odd, 0, acc);
+        step<REFILL, P1>(s, odd, even, 0, odd, k + KTURN + KODD, acc);
+      }
+    }
+    if (PARTS == 1 && k < s.k_last) {
+      step<PLAIN, 0>(s, even, even, 1, even, 0, acc);
+      step<LAST, 0>(s, even, even, 0, even, 0, acc);
     }
     // zeros still on their way must not land in what comes after
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

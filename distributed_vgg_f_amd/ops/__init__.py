@@ -15,6 +15,9 @@ from . import cpu_ref
 from . import native  # noqa: F401  (re-export for engine / tests)
 
 
+_ACT_ID = {name: i for i, name in enumerate(cpu_ref.ACTIVATIONS)}
+
+
 def conv2d(x, w, bias=None, stride: int = 1, pad: int = 0, relu: bool = False):
     if x.is_cuda:
         from .autograd import ConvFunction
@@ -55,20 +58,16 @@ def gated_linear(x, w_gate, w_up, bias_gate=None, bias_up=None,
         return dropout(h, p, seed, offset)
     if x.dim() < 1:
         raise ValueError("gated_linear: x must have a last dimension")
-    rows = math.prod(x.shape[:-1])
-    args = (x.reshape(rows, x.shape[-1]), w_gate, w_up, bias_gate, bias_up)
-    act_id = list(cpu_ref.ACTIVATIONS).index(act)
-    p = max(float(p), 0.0)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in args):
-        from .autograd import GatedLinearFunction
-        h = GatedLinearFunction.apply(*args, act_id, p, seed, offset)
-    else:
-        on_device = isinstance(offset, torch.Tensor)
-        h = native.ext().gated_fwd(*args, act_id, p, seed,
-                                   0 if on_device else offset,
-                                   offset if on_device else None)[0]
-    return h.view(*x.shape[:-1], h.shape[-1])
+    flat = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]),
+                                            x.shape[-1])
+    on_device = isinstance(offset, torch.Tensor)
+    h = native.ext().gated_linear(
+        flat, w_gate, w_up, bias_gate, bias_up, _ACT_ID[act], max(p, 0.0),
+        seed, 0 if on_device else offset, offset if on_device else None,
+        # direct-grad: arena views attached by ArenaOptimizer
+        [getattr(t, "_dvgg_gbuf", None)
+         for t in (w_gate, w_up, bias_gate, bias_up)])
+    return h if x.dim() == 2 else h.view(*x.shape[:-1], h.shape[-1])
 
 
 def lrn(x, size: int = 5, alpha: float = 1e-4, beta: float = 0.75, k: float = 2.0):
@@ -105,8 +104,9 @@ def dropout(x, p: float, seed: int = 0, offset: Union[int, torch.Tensor] = 0,
         return x.masked_fill(torch.ones((), dtype=torch.bool,
                                         device=x.device), 0.0)
     if x.is_cuda:
-        from .autograd import DropoutFunction
-        return DropoutFunction.apply(x, float(p), seed, offset)
+        if isinstance(offset, torch.Tensor):
+            return native.ext().dropout(x, p, seed, 0, offset)
+        return native.ext().dropout(x, p, seed, offset)
     if mask is None:
         gen = torch.Generator().manual_seed(int(seed + offset))
         mask = (torch.rand(x.shape, generator=gen) >= p).to(x.dtype)

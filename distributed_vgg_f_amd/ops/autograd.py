@@ -1,6 +1,7 @@
 """Custom autograd Functions wrapping the HIP kernels (GPU path only).
 
-Each Function mirrors one K# row of SURVEY.md section 2.4. The CPU path never
+Each Function mirrors one K# row of SURVEY.md section 2.4 (those of dropout
+and of the gated unit are in csrc/fn.cpp). The CPU path never
 reaches these — layers dispatch CPU tensors to ops.cpu_ref compositions and
 let torch autograd differentiate those. Here, forward/backward both call
 hand-written CDNA4 kernels via ops.native.ext().
@@ -102,39 +103,6 @@ class LinearFunction(torch.autograd.Function):
         return dx, _fresh(dw), _fresh(db), None
 
 
-class GatedLinearFunction(torch.autograd.Function):
-    """act(x w_gate + b_gate) * (x w_up + b_up) and its dropout. Keeps both
-    projections; backward is one pass over them and two products."""
-
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, act: int, p: float,
-                seed: int, offset):
-        on_device = isinstance(offset, torch.Tensor)
-        h, *saved = _ext().gated_fwd(
-            x, w_gate, w_up, bias_gate, bias_up, act, p, seed,
-            0 if on_device else offset, offset if on_device else None, True)
-        ctx.save_for_backward(*saved)
-        ctx.args = act, p, seed, 0 if on_device else offset
-        ctx.shape = w_gate.shape
-        # direct-grad: arena views attached by ArenaOptimizer
-        ctx.outs = [None] + [getattr(t, "_dvgg_gbuf", None)
-                             for t in (w_gate, w_up, bias_gate, bias_up)]
-        return h
-
-    @staticmethod
-    def backward(ctx, dh):
-        if torch.is_grad_enabled():     # the gradients' own graph is wanted
-            raise RuntimeError("gated_linear differentiates once: no "
-                               "create_graph=True through it")
-        gu, x, w_gate, w_up, *used = ctx.saved_tensors
-        need = sum(1 << i for i in range(5) if ctx.needs_input_grad[i])
-        grads = _ext().gated_bwd(dh, gu, x, w_gate, w_up, *ctx.shape,
-                                 *ctx.args, used[0] if used else None, need,
-                                 ctx.outs)
-        return (grads[0], *(_fresh(g) for g in grads[1:]),
-                None, None, None, None)
-
-
 class LRNFunction(torch.autograd.Function):
     """K4/K5. Fwd saves only x: backward recomputes the window scale s
     (cheap FMAs over the x it reloads anyway) and sb/snb via the same
@@ -173,29 +141,6 @@ class MaxPoolFunction(torch.autograd.Function):
         dx = _ext().maxpool_bwd(dy.contiguous(), idx, H, W, kernel, stride,
                                 pad_l, pad_r)
         return dx, None, None, None, None
-
-
-class DropoutFunction(torch.autograd.Function):
-    """K12: Philox counter-based mask that is never stored: backward draws
-    it again from (p, seed, offset) and runs the forward's kernel on dy."""
-
-    @staticmethod
-    def forward(ctx, x, p: float, seed: int, offset):
-        ctx.p, ctx.seed, ctx.offset = p, seed, offset
-        if not isinstance(offset, torch.Tensor):
-            return _ext().dropout(x.contiguous(), p, seed, offset)[0]
-        # the kernel keeps a copy of the offset that it drew with: the
-        # caller may count the tensor up before backward runs
-        y, used = _ext().dropout(x.contiguous(), p, seed, 0, offset)
-        ctx.offset = None
-        ctx.save_for_backward(used)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        offset = ctx.offset if ctx.offset is not None else ctx.saved_tensors[0]
-        return DropoutFunction.apply(dy, ctx.p, ctx.seed, offset), None, \
-            None, None
 
 
 class SoftmaxXentFunction(torch.autograd.Function):
