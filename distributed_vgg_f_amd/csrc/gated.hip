@@ -327,24 +327,43 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
 }
 
 // ------------------------------------------------- joining a split product
-// Sums the slabs in their order (the same result every time), 8 columns a
-// thread.
-template <class T>
+// Sums the slabs in a fixed order (the same result every time), 8 columns a
+// thread; WIDE, for few columns and many slabs: 8 threads, each an eighth of
+// the slabs (one row of 25088 x 64 in 49 slabs: 21.5 -> 9.3 us
+// with its product).
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void join_gated_kernel(
     const float* __restrict__ slab, int splits, i64 slab_ld, OutArgs o) {
   const u32 off = o.drop ? o.d.off() : 0;
   const int per = int(slab_ld / 8);
-  const i64 one = (i64)o.M * slab_ld;
-  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < (i64)o.M * per;
-       c += (i64)gridDim.x * 256) {
-    const float* sp = slab + c * 8;
+  const i64 one = (i64)o.M * slab_ld, chunks = (i64)o.M * per;
+  constexpr int LANES = WIDE ? 8 : 1;   // threads of a chunk, 8 lanes apart
+  const int lane = threadIdx.x & 63, mine = WIDE ? lane >> 3 : 0;
+  const i64 first = (i64)blockIdx.x * (blockDim.x / LANES) +
+                    (WIDE ? (threadIdx.x >> 6) * 8 + (lane & 7)
+                          : threadIdx.x);
+  // whole waves stay together: the threads of a chunk exchange their sums
+  for (i64 c = first; c - (WIDE ? lane & 7 : 0) < chunks;
+       c += (i64)gridDim.x * (blockDim.x / LANES)) {
+    const bool in = c < chunks;
+    const float* sp = slab + (in ? c : 0) * 8 + mine * 2 * one;
     f32x8 g{}, u{};
-#pragma unroll 2
-    for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+    for (int s = mine; s < splits; s += LANES) {
       g += load8f(sp);
       u += load8f(sp + one);
-      sp += 2 * one;
+      sp += 2 * LANES * one;
     }
+    if (WIDE) {
+#pragma unroll
+      for (int d = 8; d < 64; d *= 2)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          g[r] += __shfl_xor(g[r], d);
+          u[r] += __shfl_xor(u[r], d);
+        }
+    }
+    if (!in || mine) continue;
     int m = int(c / per);
     finish8<T>(o, off, m, int(c - (i64)m * per) * 8, g, u);
   }
@@ -366,6 +385,148 @@ __global__ __launch_bounds__(256) void join_plain_kernel(
     int n = int(c - m * per) * 8;
     u16* out = m < rows ? c0 + m * cols : c1 + (m - rows) * cols;
     store8(out, n, cols, round8<T>(v));
+  }
+}
+
+// ------------------------------------------------- few rows: the weights
+// Up to 16 rows of X: the forward pass is one reading of both weights, and a
+// tile's way through LDS only delays it. Here a wave takes 128 columns of
+// each weight and a part of the contraction and loads 32 k of them straight
+// into registers: lane (c, q) = (lane % 16, lane / 16) rows 8 q .. 8 q + 7 of
+// columns 8 c .. 8 c + 7. Eight rows of eight columns are turned over by
+// v_perm into eight fragments, one for each column j of the eight, of which
+// lane (c, q) holds column 8 c + j and its 8 k: what the matrix instruction
+// takes. The next 32 k are on their way meanwhile (32 KB a wave). The four
+// waves of a block, each with its part of the contraction, meet in LDS; parts
+// of several blocks meet in join_gated_kernel.
+struct RowsArgs {
+  const u16* x;
+  const u16* w[2];
+  i64 ldx, ldw;
+  int M, K, N;
+  int splits;
+  float* slab;          // [splits][2][M][slab_ld] if splits > 1
+  i64 slab_ld;
+  OutArgs out;
+};
+
+typedef __attribute__((ext_vector_type(4))) u32 u32x4v;
+
+DEV s16x8 pick_column(const u32x4v (&w)[8], int j) {
+  u32x4v f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    f[t] = __builtin_amdgcn_perm(w[2 * t + 1][j / 2], w[2 * t][j / 2],
+                                 j & 1 ? 0x07060302u : 0x05040100u);
+  return __builtin_bit_cast(s16x8, f);
+}
+DEV f32x4 mfma_of(s16x8 a, s16x8 b, f32x4 c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+      0);
+}
+DEV f32x4 mfma_of(s16x8 a, s16x8 b, f32x4 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void rows_kernel(RowsArgs p) {
+  __shared__ __attribute__((aligned(16))) float red[4][2][16][128];
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 128, split = blockIdx.y;
+
+  // steps of 32 k: [first, last) of this wave
+  const int steps = (p.K + 31) / 32, parts = p.splits * 4;
+  const int part = split * 4 + wave;
+  const int each_ = steps / parts, more = steps % parts;
+  const int first = part * each_ + min(part, more);
+  const int last = first + each_ + (part < more);
+
+  const u32 ldw2 = u32(p.ldw) * 2;
+  const bool col_in = n0 + c * 8 < p.N, row_in = c < p.M;
+  u32 woff[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    woff[r] = col_in ? (8 * q + r) * ldw2 + c * 16 : OUT_OF_RANGE;
+  const u32 xoff = u32(c) * u32(p.ldx) * 2 + q * 16;
+
+  u32x4v w[2][2][8];    // [buffer][weight][row]
+  u32x4v xf[2];
+  auto fetch = [&](int b, int step) {
+    const int k = step * 32;
+    // an empty buffer behind this wave's part: zeros, no memory moves
+    const int rows = step < last ? min(p.K - k, 32) : 0;
+    const u32 bytes = rows * ldw2 - min(rows, 1) * n0 * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<u16*>(uniform(p.w[h] + (i64)k * p.ldw + n0)), 0,
+          uniform(bytes), 0x00020000);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        w[b][h][r] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, woff[r], 0,
+                                                           0);
+    }
+    const u32 xbytes = rows > 0 ? u32(p.M - 1) * u32(p.ldx) * 2 +
+                                      ((rows + 7) & ~7) * 2 : 0;
+    auto rx = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<u16*>(uniform(p.x + k)), 0, uniform(xbytes), 0x00020000);
+    xf[b] = __builtin_amdgcn_raw_buffer_load_b128(
+        rx, row_in && q * 8 < rows ? xoff : OUT_OF_RANGE, 0, 0);
+  };
+  f32x4 acc[2][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](int b) {
+    const s16x8 x = __builtin_bit_cast(s16x8, xf[b]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        acc[h][j] = mfma_of(pick_column(w[b][h], j), x, acc[h][j], T());
+  };
+  fetch(0, first);
+  for (int step = first; step < last; step += 2) {
+    fetch(1, step + 1);
+    multiply(0);
+    fetch(0, step + 2);
+    multiply(1);
+  }
+
+  // lane: row c of X, columns 8 (4 q + r) + j
+  if (row_in) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float* d = &red[wave][h][c][(4 * q + r) * 8];
+        f32x8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = acc[h][j][r];
+        store8f(d, v);
+      }
+  }
+  __syncthreads();
+  const u32 off = p.out.drop ? p.out.d.off() : 0;
+  for (int i = threadIdx.x; i < p.M * 16; i += 256) {
+    const int m = i / 16, n = n0 + i % 16 * 8;
+    if (n >= p.N) continue;
+    f32x8 g = load8f(&red[0][0][m][i % 16 * 8]);
+    f32x8 u = load8f(&red[0][1][m][i % 16 * 8]);
+#pragma unroll
+    for (int v = 1; v < 4; ++v) {
+      g += load8f(&red[v][0][m][i % 16 * 8]);
+      u += load8f(&red[v][1][m][i % 16 * 8]);
+    }
+    if (p.splits == 1) {
+      finish8<T>(p.out, off, m, n, g, u);
+    } else {
+      float* sp = p.slab + ((i64)split * 2 * p.M + m) * p.slab_ld + n;
+      store8f(sp, g);
+      store8f(sp + (i64)p.M * p.slab_ld, u);
+    }
   }
 }
 
@@ -528,6 +689,8 @@ static i64 ld_of(const at::Tensor& t) {
   return t.size(0) == 1 ? t.size(1) : t.stride(0);
 }
 
+constexpr int ROWS_MAX = 16, ROWS_TARGET = 256;
+
 struct Plan { int fm, fn, splits, tiles_m, tiles_n, stages; bool brief; };
 
 // Which tile, and into how many parts the contraction is split: the least
@@ -557,7 +720,9 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
     const int tm = ceil_div(rows, 32 * k.fm);
     const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
                    (mode == WGRAD ? 2 : 1);
-    for (int sp = 1; sp <= stages && sp <= 32; sp += sp < 4 ? 1 : sp / 2) {
+    // 1 2 3 4 6 8 12 16 24 32
+    for (int sp = 1; sp <= stages && sp <= 32;
+         sp += sp < 4 ? 1 : sp & (sp - 1) ? sp / 3 : sp / 2) {
       const double wgs = double(tm) * tn * sp, slots = CUS * k.per_cu;
       const double depth = ceil_div(stages, sp) * parts;
       auto round = [&](double n) {
@@ -602,6 +767,26 @@ static void launch(const Plan& pl, const ProductArgs& a) {
   TORCH_CHECK(false, "gated_linear: no tile of this size");
 }
 
+template <class T>
+static void join_gated_of(const float* slab, int splits, i64 slab_ld,
+                          const OutArgs& out) {
+  i64 chunks = (i64)out.M * slab_ld / 8;
+  const bool wide = splits >= 8 && chunks < 8192;
+  // few chunks: a wave a block, so that they reach more CUs
+  const int threads = chunks < 65536 ? 64 : 256;
+  const int per = wide ? threads / 8 : threads;
+  dim3 grid(u32(std::min<i64>((chunks + per - 1) / per, 8192)));
+  auto kernel = wide ? join_gated_kernel<T, true> : join_gated_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, cur_stream(), slab,
+                     splits, slab_ld, out);
+  HIP_CHECK(hipGetLastError());
+}
+static void join_gated(bool half, const float* slab, int splits, i64 slab_ld,
+                       const OutArgs& out) {
+  if (half) join_gated_of<_Float16>(slab, splits, slab_ld, out);
+  else join_gated_of<__bf16>(slab, splits, slab_ld, out);
+}
+
 template <int MODE>
 static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
                     const at::TensorOptions& opt) {
@@ -621,17 +806,14 @@ static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
   if (half) launch<_Float16, MODE>(pl, a);
   else launch<__bf16, MODE>(pl, a);
   if (pl.splits == 1) return;
+  if (MODE == FWD) {
+    join_gated(half, a.slab, pl.splits, a.slab_ld, a.out);
+    return;
+  }
   i64 chunks = (i64)a.rows * (MODE == WGRAD ? 2 : 1) * a.slab_ld / 8;
   dim3 grid(u32(std::min<i64>((chunks + 255) / 256, 8192)));
   auto st = cur_stream();
-  if (MODE == FWD) {
-    if (half)
-      hipLaunchKernelGGL(join_gated_kernel<_Float16>, grid, dim3(256), 0, st,
-                         a.slab, pl.splits, a.slab_ld, a.out);
-    else
-      hipLaunchKernelGGL(join_gated_kernel<__bf16>, grid, dim3(256), 0, st,
-                         a.slab, pl.splits, a.slab_ld, a.out);
-  } else if (half) {
+  if (half) {
     hipLaunchKernelGGL(join_plain_kernel<_Float16>, grid, dim3(256), 0, st,
                        a.slab, pl.splits, a.slab_ld, a.rows, a.cols, mats,
                        a.c[0], a.c[1]);
@@ -641,6 +823,35 @@ static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
                        a.c[0], a.c[1]);
   }
   HIP_CHECK(hipGetLastError());
+}
+
+// Few rows: about one block a CU (12 x 9216 x 4096: 37.0 us; 128 blocks 43.0,
+// 512 38.7, 1024 46.3), and at least 2 steps of 32 k a wave. Letting the last
+// block of a column join the parts in place of a second kernel took 23.8 us
+// instead of 19.1 for one row of 4096 x 4096: what it waits for, the caches
+// of eight XCDs written back, costs more than a launch.
+static void product_rows(at::ScalarType type, const ProductArgs& a,
+                         const at::TensorOptions& opt) {
+  RowsArgs p{a.a[0], {a.b[0], a.b[1]}, a.lda, a.ldb, a.rows, a.k_len, a.cols,
+             1, nullptr, up(a.cols, 8), a.out};
+  const int blocks = ceil_div(a.cols, 128);
+  p.splits = int(std::max<i64>(
+      1, std::min<i64>(ROWS_TARGET / blocks, a.k_len / (32 * 4 * 2))));
+  at::Tensor slab;
+  if (p.splits > 1) {
+    slab = at::empty({(i64)p.splits * 2 * a.rows * p.slab_ld},
+                     opt.dtype(at::kFloat));
+    p.slab = slab.data_ptr<float>();
+  }
+  const bool half = type == at::kHalf;
+  auto st = cur_stream();
+  dim3 grid(blocks, p.splits);
+  if (half)
+    hipLaunchKernelGGL(rows_kernel<_Float16>, grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL(rows_kernel<__bf16>, grid, dim3(256), 0, st, p);
+  HIP_CHECK(hipGetLastError());
+  if (p.splits > 1) join_gated(half, p.slab, p.splits, p.slab_ld, a.out);
 }
 
 static void check_operand(const at::Tensor& t, const char* name,
@@ -735,7 +946,8 @@ std::vector<at::Tensor> gated_fwd(
     a.out = OutArgs{mptr(h), train ? gu.data_ptr<float>() : nullptr,
                     {bg ? cptr(bgc) : nullptr, bu ? cptr(buc) : nullptr},
                     int(M), int(N), ldg, int(act), p > 0.0, d};
-    product<FWD>(type, make_plan(FWD, M, N, K), a, x.options());
+    if (M <= ROWS_MAX) product_rows(type, a, x.options());
+    else product<FWD>(type, make_plan(FWD, M, N, K), a, x.options());
   }
   if (!train) return {h};
   std::vector<at::Tensor> r{h, gu, xl, gl, ul};
