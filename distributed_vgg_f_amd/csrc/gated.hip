@@ -192,7 +192,7 @@ struct ProductArgs {
   i64 lda, ldb;
   int rows, cols;       // of one output matrix
   int k_len;
-  int splits, stages;   // stages of one part of the contraction
+  int splits, stages;   // stages of 64 k of one part of the contraction
   int tiles_m, tiles_n;
   float* slab;          // [splits][2 or 1][rows][slab_ld] if splits > 1
   i64 slab_ld;          // cols rounded up to 8
@@ -228,11 +228,11 @@ DEV void emit_gated(const ProductArgs& p, int split, u32 off, int m, int n,
   }
 }
 
-template <class T, int MODE, int FM, int FN, bool SHORT = false>
+template <class T, int MODE, int FM, int FN, int BK, bool SHORT = false>
 __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
   constexpr bool ATR = MODE == WGRAD, BTR = MODE != DGRAD;
-  using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN, MODE == FWD,
-                  SHORT>;
+  using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN, BK,
+                  MODE == FWD, SHORT>;
   // two objects, so that reads of one do not wait for loads into the other
   __shared__ __attribute__((aligned(1024))) char even[TL::STAGE];
   __shared__ __attribute__((aligned(1024))) char odd[SHORT ? 16 : TL::STAGE];
@@ -275,8 +275,8 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
     s.b[1][1] = s.b[1][0] + bh;
   }
   const int q = p.stages / p.splits, r = p.stages % p.splits;
-  s.k_first = (split * q + min(split, r)) * TILE_BK;
-  s.k_last = min(s.k_first + (q + (split < r)) * TILE_BK, p.k_len);
+  s.k_first = (split * q + min(split, r)) * 64;
+  s.k_last = min(s.k_first + (q + (split < r)) * 64, p.k_len);
 
   f32x4 acc[FM][FN];
   TL tile;
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
   // Through LDS, some rows of a wave at a time: the lanes then hold whole
   // stretches of a row (128 bytes a store and more), and one copy of the
   // epilogue's code for these rows is enough.
-  constexpr int ROWS = SHORT ? 16 : 32;
+  constexpr int ROWS = SHORT || BK == 32 ? 16 : 32;
   constexpr int PITCH = 16 * FN + 4;      // floats; + 4: rows change banks
   constexpr int MINE = SHORT ? TL::STAGE / 4 : TL::STAGE / 2;
   static_assert(ROWS * PITCH * 4 <= MINE, "a wave's part of the LDS");
@@ -691,7 +691,7 @@ static i64 ld_of(const at::Tensor& t) {
 
 constexpr int ROWS_MAX = 16, ROWS_TARGET = 256;
 
-struct Plan { int fm, fn, splits, tiles_m, tiles_n, stages; bool brief; };
+struct Plan { int fm, fn, bk, splits, tiles_m, tiles_n, stages; bool brief; };
 
 // Which tile, and into how many parts the contraction is split: the least
 // time by a model of what the tiles measured over 44 products from 1 x 512 to
@@ -700,13 +700,14 @@ struct Plan { int fm, fn, splits, tiles_m, tiles_n, stages; bool brief; };
 // Microseconds. A stage costs `one` if a tile has its CU to itself and `all`
 // if the CU is full; `edge` is a tile's first loads and its epilogue.
 static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
-  struct Kind { int fm, fn, per_cu; double one, all, edge; bool brief; };
-  static const Kind kinds[] = {{8, 8, 1, 1.24, 1.24, 9.8, false},
-                               {4, 4, 2, 0.69, 0.96, 3.9, false},
-                               {2, 4, 3, 0.61, 0.93, 2.8, false},
-                               {4, 4, 3, 0.69, 0.96, 3.9, true}};
+  struct Kind { int fm, fn, bk, per_cu; double one, all, edge; bool brief; };
+  static const Kind kinds[] = {{8, 8, 64, 1, 1.24, 1.24, 9.8, false},
+                               {4, 4, 64, 2, 0.69, 0.96, 3.9, false},
+                               {2, 4, 64, 3, 0.61, 0.93, 2.8, false},
+                               {4, 4, 32, 4, 0.69, 1.85, 4.0, false},
+                               {4, 4, 64, 4, 0.69, 1.85, 3.9, true}};
   constexpr double CUS = 256, MEM = 4.5e6, JOIN = 2.8, JOIN_MEM = 7e6;
-  const int stages = ceil_div(k_len, TILE_BK);
+  const int stages = ceil_div(k_len, 64);
   const double mats = mode == DGRAD ? 1 : 2, parts = mode == DGRAD ? 2 : 1;
   const double out = double(rows) * cols;
   // bytes that the product moves at least
@@ -716,6 +717,10 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
   Plan best{};
   double least = 0;
   for (const Kind& k : kinds) {
+    // Stages of 32 k pay only where both operands lie along their rows, and
+    // contractions are short (256 x 9216 x 4096: 73.5 -> 60.3 us); else their
+    // rows of 64 bytes cost more than four tiles a CU gain.
+    if (k.bk == 32 && mode != WGRAD) continue;
     if (k.brief && (mode != WGRAD || stages > 1)) continue;
     const int tm = ceil_div(rows, 32 * k.fm);
     const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
@@ -736,7 +741,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
       if (sp > 1) t += JOIN + sp * mats * out * 8 / JOIN_MEM;
       if (least == 0 || t < least) {
         least = t;
-        best = Plan{k.fm, k.fn, sp, tm, tn, stages, k.brief};
+        best = Plan{k.fm, k.fn, k.bk, sp, tm, tn, stages, k.brief};
       }
     }
   }
@@ -748,21 +753,22 @@ static void launch(const Plan& pl, const ProductArgs& a) {
   dim3 grid(u32(pl.tiles_m) * pl.tiles_n * pl.splits);
   auto st = cur_stream();
   if (pl.brief) {
-    hipLaunchKernelGGL((product_kernel<T, WGRAD, 4, 4, true>), grid,
+    hipLaunchKernelGGL((product_kernel<T, WGRAD, 4, 4, 64, true>), grid,
                        dim3(256), 0, st, a);
     HIP_CHECK(hipGetLastError());
     return;
   }
-#define TILE_CASE(FM, FN)                                                  \
-  if (pl.fm == FM && pl.fn == FN) {                                        \
-    hipLaunchKernelGGL((product_kernel<T, MODE, FM, FN>), grid, dim3(256), \
-                       0, st, a);                                          \
+#define TILE_CASE(FM, FN, BK)                                              \
+  if (pl.fm == FM && pl.fn == FN && pl.bk == BK) {                         \
+    hipLaunchKernelGGL((product_kernel<T, MODE, FM, FN, BK>), grid,        \
+                       dim3(256), 0, st, a);                               \
     HIP_CHECK(hipGetLastError());                                          \
     return;                                                                \
   }
-  TILE_CASE(8, 8)
-  TILE_CASE(4, 4)
-  TILE_CASE(2, 4)
+  TILE_CASE(8, 8, 64)
+  TILE_CASE(4, 4, 64)
+  TILE_CASE(2, 4, 64)
+  if constexpr (MODE == WGRAD) { TILE_CASE(4, 4, 32) }
 #undef TILE_CASE
   TORCH_CHECK(false, "gated_linear: no tile of this size");
 }

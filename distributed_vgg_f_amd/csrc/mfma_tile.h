@@ -10,7 +10,7 @@
 // 32 k a wave reads 16 (FM + FN) rows of 64 bytes for FM FN products of 16
 // cycles, 64 B/cycle of the CU's 128 at 8 x 8, but 96 for 8 waves of 8 x 4.
 //
-// Stages of 64 k go straight from memory to LDS (16 bytes a lane), two deep;
+// Stages of 64 (or 32) k go straight from memory to LDS (16 bytes a lane), two deep;
 // the fragments of the next 32 k are read while the present ones multiply, so
 // a stage costs one barrier. Buffer loads put zeros where rows, columns or
 // the contraction end.
@@ -58,7 +58,6 @@ DEV void mfma_done(f32x4 (&c)[FM][FN]) {
 
 using u64 = unsigned long long;
 
-constexpr int TILE_BK = 64;
 constexpr u32 OUT_OF_RANGE = 0x80000000u;   // no buffer here reaches it
 
 // A value that all lanes share, in a scalar register: the compiler does not
@@ -71,19 +70,19 @@ DEV const u16* uniform(const u16* p) {
       u64(uniform(u32(v >> 32))) << 32 | uniform(u32(v)));
 }
 
-// One half of an operand's rows in one stage: ROWS rows x 64 k.
-template <bool TR, int ROWS>
+// One half of an operand's rows in one stage: ROWS rows x BK k (64 or 32).
+template <bool TR, int ROWS, int BK>
 struct Panel {
-  static constexpr int BYTES = ROWS * TILE_BK * 2;
+  static constexpr int BYTES = ROWS * BK * 2;
   static constexpr int LOADS = BYTES / 4096;    // 16-byte loads a thread
-  static constexpr int PITCH = TR ? ROWS * 2 : TILE_BK * 2;
+  static constexpr int PITCH = TR ? ROWS * 2 : BK * 2;
 
   // 16-byte segments (TR = false) trade places by row so that the 16 rows
   // that a fragment reads together fall into 16 different bank groups.
   // TR = true: 32-byte chunks trade places by k so that the 4 + 4 rows of k
   // that two 16-lane groups read together do.
   DEV static int swz(int r) {
-    if (!TR) return (r >> 1) & 7;
+    if (!TR) return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
     if (ROWS >= 128) return (r & 3) | ((r >> 3) & 1) << 2;
     return ((r >> 1) & 1) | ((r >> 3) & 1) << 1;
   }
@@ -109,7 +108,7 @@ struct Panel {
                 int k_left, int wave, int i) const {
     // rows of memory are whole vectors: a last one that the operand fills
     // in part is followed by its padding
-    const int kk = max(min(k_left, TILE_BK), 0);
+    const int kk = max(min(k_left, BK), 0);
     const int rr = max(min(rows_left, ROWS), 0);
     const int outer = TR ? kk : rr, inner = ((TR ? rr : kk) + 7) & ~7;
     const u32 bytes = min(outer, 1) * min(inner, 1) *
@@ -124,18 +123,19 @@ struct Panel {
 
 // Reads a wave's fragments out of a panel: F fragments of 16 rows from row
 // `first` (a multiple of 16 * F, or of 64).
-template <bool TR, int ROWS, int F>
+template <bool TR, int ROWS, int BK, int F>
 struct Frags {
+  using P = Panel<TR, ROWS, BK>;
   u32 addr[TR ? F : 1];
   DEV void init(int lane, int first) {
     if (!TR) {
       int r = first + (lane & 15);
-      addr[0] = r * 128 + (((lane >> 4) ^ Panel<TR, ROWS>::swz(r)) << 4);
+      addr[0] = r * BK * 2 + (((lane >> 4) ^ P::swz(r)) << 4);
     } else {
       int k = (lane >> 4) * 8 + ((lane & 15) >> 2);
 #pragma unroll
       for (int j = 0; j < F; ++j) {
-        int chunk = (first / 16 + j) ^ Panel<TR, ROWS>::swz(k);
+        int chunk = (first / 16 + j) ^ P::swz(k);
         addr[j] = k * ROWS * 2 + chunk * 32 + (lane & 3) * 8;
       }
     }
@@ -143,7 +143,7 @@ struct Frags {
   DEV s16x8 read(const lds_char* panel, int j, int half) const {
     if (!TR) {
       u32 a = addr[0] ^ (half << 6);
-      return *(const lds_s16x8*)(panel + a + j * 2048);
+      return *(const lds_s16x8*)(panel + a + j * 32 * BK);
     }
     const lds_char* p = panel + addr[j] + half * 32 * ROWS * 2;
     s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
@@ -164,23 +164,26 @@ struct TileSrc {
   int k_first, k_last;      // the contraction [k_first, k_last) of each part
 };
 
+// BK: k of a stage. Stages of 64 take a barrier for every two steps of 32
+// and keep rows of 128 bytes together; stages of 32 take half the LDS, and
+// more tiles share a CU.
 // PAIRED: a wave takes the same columns of both halves, else all columns of
 // one. SHORT: the whole contraction is one stage, which then is all the LDS
 // that the tile needs; more tiles share a CU.
-template <class T, bool ATR, bool BTR, int PARTS, int FM, int FN, bool PAIRED,
-          bool SHORT>
+template <class T, bool ATR, bool BTR, int PARTS, int FM, int FN, int BK,
+          bool PAIRED, bool SHORT>
 struct Tile {
   static constexpr int BM = 32 * FM, BN = 32 * FN, HALF = BN / 2;
-  using PA = Panel<ATR, BM>;
-  using PB = Panel<BTR, HALF>;
+  using PA = Panel<ATR, BM, BK>;
+  using PB = Panel<BTR, HALF, BK>;
   static constexpr int STAGE = PA::BYTES + 2 * PB::BYTES;
   static constexpr int LOADS = PA::LOADS + 2 * PB::LOADS;
   static constexpr int FH = PAIRED ? FN / 2 : FN;  // fragments in a half
 
   PA pa;
   PB pb[2];
-  Frags<ATR, BM, FM> ra;
-  Frags<BTR, HALF, FH> rb;
+  Frags<ATR, BM, BK, FM> ra;
+  Frags<BTR, HALF, BK, FH> rb;
   s16x8 fa[FM], fb[FN];
   int wave;
 
@@ -212,15 +215,16 @@ struct Tile {
   // and issues in 4: bunched up, the others would hold it up):
   //   - the read of each fragment's successor behind its last use, from half
   //     `half` of `src` (LAST: there is none). That of A's last row comes in
-  //     the next step, so this one begins with its own, from `cur`;
-  //   - REFILL, the half that changes over to the next stage: after its first
+  //     the next step, so this one begins with its own, from `cur`, `own`;
+  //   - REFILL, the step that changes over to the next stage: after its first
   //     rows every wave is done reading `dst` and its own loads into `src`
   //     have landed, so it syncs there, with products still queued; then the
   //     loads that refill `dst`.
   enum Kind { PLAIN, REFILL, LAST };
   template <Kind KIND, int PART>
-  DEV void step(const TileSrc& s, const lds_char* cur, const lds_char* src,
-                int half, lds_char* dst, int k, f32x4 (&acc)[FM][FN]) {
+  DEV void step(const TileSrc& s, const lds_char* cur, int own,
+                const lds_char* src, int half, lds_char* dst, int k,
+                f32x4 (&acc)[FM][FN]) {
     constexpr bool FILL = KIND == REFILL;
     constexpr int ROW0 = !FILL ? 0 : FM > 2 ? 2 : 1;    // first row of reads
     constexpr int SLOTS = (FM > 2 ? FM - 1 - ROW0 : 1) * FN;
@@ -229,7 +233,7 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         mfma32<T>(acc[i][j], fb[j], fa[i]);
-        if (i == 0 && j == 1) fetch_a(cur, half ^ 1, FM - 1);
+        if (i == 0 && j == 1) fetch_a(cur, own, FM - 1);
         if (KIND != LAST && i >= ROW0) {
           if (j == 1 && i > 0) fetch_a(src, half, i - 1);
           if (j == 3 && i == 2 && ROW0 == 2) fetch_a(src, half, 0);
@@ -262,8 +266,9 @@ struct Tile {
   DEV void run(lds_char* even, lds_char* odd, const TileSrc& s, int wave_,
                int lane, f32x4 (&acc)[FM][FN]) {
     constexpr int P1 = PARTS - 1;
-    constexpr int KODD = PARTS == 2 ? 0 : TILE_BK;   // k of the odd stage
-    constexpr int KTURN = KODD + TILE_BK;            // k of a turn of two
+    constexpr int LASTH = BK / 32 - 1;          // last half of a stage
+    constexpr int KODD = PARTS == 2 ? 0 : BK;   // k of the odd stage
+    constexpr int KTURN = KODD + BK;            // k of a turn of two
     wave = wave_;
     pa.init(wave, lane, s.lda, s.rows_a);
     pb[0].init(wave, lane, s.ldb, s.rows_b[0]);
@@ -289,15 +294,15 @@ struct Tile {
     if (!SHORT) {
       // whole turns; a last single stage of one part is left for below
       for (; k < s.k_last - KODD; k += KTURN) {
-        step<PLAIN, 0>(s, even, even, 1, even, 0, acc);
-        step<REFILL, 0>(s, even, odd, 0, even, k + KTURN, acc);
-        step<PLAIN, 0>(s, odd, odd, 1, odd, 0, acc);
-        step<REFILL, P1>(s, odd, even, 0, odd, k + KTURN + KODD, acc);
+        if (BK == 64) step<PLAIN, 0>(s, even, 0, even, 1, even, 0, acc);
+        step<REFILL, 0>(s, even, LASTH, odd, 0, even, k + KTURN, acc);
+        if (BK == 64) step<PLAIN, 0>(s, odd, 0, odd, 1, odd, 0, acc);
+        step<REFILL, P1>(s, odd, LASTH, even, 0, odd, k + KTURN + KODD, acc);
       }
     }
     if (PARTS == 1 && k < s.k_last) {
-      step<PLAIN, 0>(s, even, even, 1, even, 0, acc);
-      step<LAST, 0>(s, even, even, 0, even, 0, acc);
+      if (BK == 64) step<PLAIN, 0>(s, even, 0, even, 1, even, 0, acc);
+      step<LAST, 0>(s, even, LASTH, even, 0, even, 0, acc);
     }
     // zeros still on their way must not land in what comes after
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
