@@ -192,7 +192,7 @@ struct ProductArgs {
   i64 lda, ldb;
   int rows, cols;       // of one output matrix
   int k_len;
-  int splits, stages;   // stages of 64 k of one part of the contraction
+  int splits;
   int tiles_m, tiles_n;
   float* slab;          // [splits][2 or 1][rows][slab_ld] if splits > 1
   i64 slab_ld;          // cols rounded up to 8
@@ -229,7 +229,8 @@ DEV void emit_gated(const ProductArgs& p, int split, u32 off, int m, int n,
 }
 
 template <class T, int MODE, int FM, int FN, int BK, bool SHORT = false>
-__global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
+__global__ __launch_bounds__(256, SHORT || BK == 32 ? 4 : FM == 8 ? 1 : 2)
+void product_kernel(ProductArgs p) {
   constexpr bool ATR = MODE == WGRAD, BTR = MODE != DGRAD;
   using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN, BK,
                   MODE == FWD, SHORT>;
@@ -274,9 +275,12 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductArgs p) {
     s.b[1][0] = p.b[1] + bn;
     s.b[1][1] = s.b[1][0] + bh;
   }
-  const int q = p.stages / p.splits, r = p.stages % p.splits;
-  s.k_first = (split * q + min(split, r)) * 64;
-  s.k_last = min(s.k_first + (q + (split < r)) * 64, p.k_len);
+  // parts of whole turns: two stages of 64 k, or one of each part
+  constexpr int TURN = MODE == DGRAD ? 64 : 128;
+  const int turns = (p.k_len + TURN - 1) / TURN;
+  const int q = turns / p.splits, r = turns % p.splits;
+  s.k_first = (split * q + min(split, r)) * TURN;
+  s.k_last = min(s.k_first + (q + (split < r)) * TURN, p.k_len);
 
   f32x4 acc[FM][FN];
   TL tile;
@@ -691,7 +695,7 @@ static i64 ld_of(const at::Tensor& t) {
 
 constexpr int ROWS_MAX = 16, ROWS_TARGET = 256;
 
-struct Plan { int fm, fn, bk, splits, tiles_m, tiles_n, stages; bool brief; };
+struct Plan { int fm, fn, bk, splits, tiles_m, tiles_n; bool brief; };
 
 // Which tile, and into how many parts the contraction is split: the least
 // time by a model of what the tiles measured over 44 products from 1 x 512 to
@@ -707,8 +711,9 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
                                {4, 4, 32, 4, 0.69, 1.85, 4.0, false},
                                {4, 4, 64, 4, 0.69, 1.85, 3.9, true}};
   constexpr double CUS = 256, MEM = 4.5e6, JOIN = 2.8, JOIN_MEM = 7e6;
-  const int stages = ceil_div(k_len, 64);
-  const double mats = mode == DGRAD ? 1 : 2, parts = mode == DGRAD ? 2 : 1;
+  // turns of the loop, and stages in each
+  const int turns = ceil_div(k_len, mode == DGRAD ? 64 : 128);
+  const double mats = mode == DGRAD ? 1 : 2;
   const double out = double(rows) * cols;
   // bytes that the product moves at least
   const double ab = mode == FWD ? rows + 2. * cols
@@ -721,15 +726,15 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
     // contractions are short (256 x 9216 x 4096: 73.5 -> 60.3 us); else their
     // rows of 64 bytes cost more than four tiles a CU gain.
     if (k.bk == 32 && mode != WGRAD) continue;
-    if (k.brief && (mode != WGRAD || stages > 1)) continue;
+    if (k.brief && (mode != WGRAD || k_len > 64)) continue;
     const int tm = ceil_div(rows, 32 * k.fm);
     const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
                    (mode == WGRAD ? 2 : 1);
     // 1 2 3 4 6 8 12 16 24 32
-    for (int sp = 1; sp <= stages && sp <= 32;
+    for (int sp = 1; sp <= turns && sp <= 32;
          sp += sp < 4 ? 1 : sp & (sp - 1) ? sp / 3 : sp / 2) {
       const double wgs = double(tm) * tn * sp, slots = CUS * k.per_cu;
-      const double depth = ceil_div(stages, sp) * parts;
+      const double depth = k.brief ? 1 : 2 * ceil_div(turns, sp);
       auto round = [&](double n) {
         const double share = k.per_cu > 1
             ? (std::ceil(n / CUS) - 1) / (k.per_cu - 1) : 1;
@@ -741,7 +746,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
       if (sp > 1) t += JOIN + sp * mats * out * 8 / JOIN_MEM;
       if (least == 0 || t < least) {
         least = t;
-        best = Plan{k.fm, k.fn, k.bk, sp, tm, tn, stages, k.brief};
+        best = Plan{k.fm, k.fn, k.bk, sp, tm, tn, k.brief};
       }
     }
   }
@@ -797,7 +802,6 @@ template <int MODE>
 static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
                     const at::TensorOptions& opt) {
   a.splits = pl.splits;
-  a.stages = pl.stages;
   a.tiles_m = pl.tiles_m;
   a.tiles_n = pl.tiles_n;
   a.slab_ld = up(a.cols, 8);

@@ -30,9 +30,10 @@ typedef __attribute__((address_space(3))) char lds_char;
 // where it is: through the builtin, result and addend are two registers and
 // the loop around them copies 128 and more of them a turn. In this order the
 // source is the schedule: products and the reads between them stay put.
-// The compiler knows nothing of the instruction's latency here: two products
-// on one accumulator must be 8 or more apart, and mfma_done() comes before
-// any other use of one.
+// The compiler knows nothing of the instruction's latency here: mfma_wait()
+// ends every piece of straight code with products in it, since the compiler
+// may move accumulators about where pieces join, and mfma_done() comes before
+// any use. tests/test_accumulator_waits.py looks at what was built.
 template <class T>
 DEV void mfma32(f32x4& c, s16x8 a, s16x8 b);
 template <>
@@ -45,11 +46,15 @@ DEV void mfma32<_Float16>(f32x4& c, s16x8 a, s16x8 b) {
   asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0"
                : "+a"(c) : "v"(a), "v"(b));
 }
+// 8 passes: 11 wait states before another instruction may touch the result
+DEV void mfma_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 10");
+  __builtin_amdgcn_sched_barrier(0);
+}
 template <int FM, int FN>
 DEV void mfma_done(f32x4 (&c)[FM][FN]) {
-  // 8 passes of 4 cycles: 11 wait states before a vector instruction may
-  // read the result, 32 here
-  asm volatile("s_nop 15\n\ts_nop 15");
+  mfma_wait();
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -153,6 +158,8 @@ struct Frags {
   }
 };
 
+constexpr int max_(int a, int b) { return a > b ? a : b; }
+
 // What one tile multiplies. The contraction may come in two parts with
 // memory of their own (dG Wg^T + dU Wu^T): their stages take turns. So may
 // the two halves of the tile's columns (X Wg | X Wu).
@@ -184,7 +191,9 @@ struct Tile {
   PB pb[2];
   Frags<ATR, BM, BK, FM> ra;
   Frags<BTR, HALF, BK, FH> rb;
-  s16x8 fa[FM], fb[FN];
+  // B's fragments twice where registers allow, of this step and of the next
+  static constexpr int SETS = FM * FN >= 64 ? 2 : 1;
+  s16x8 fa[FM], fb[SETS][FN];
   int wave;
 
   // Loads number `i` of a stage. Behind the last k the buffers are empty:
@@ -205,44 +214,56 @@ struct Tile {
   DEV void fetch_a(const lds_char* src, int half, int i) {
     fa[i] = ra.read(src, i, half);
   }
-  DEV void fetch_b(const lds_char* src, int half, int j) {
+  DEV void fetch_b(const lds_char* src, int half, int set, int j) {
     const int h = PAIRED ? j / FH : wave & 1;
-    fb[j] = rb.read(src + PA::BYTES + h * PB::BYTES, j % FH, half);
+    fb[set][j] = rb.read(src + PA::BYTES + h * PB::BYTES, j % FH, half);
   }
 
-  // 32 k: the products of the fragments at hand, row by row of A. Between
-  // them, one or two at a time (a product keeps the matrix core for 16 cycles
-  // and issues in 4: bunched up, the others would hold it up):
-  //   - the read of each fragment's successor behind its last use, from half
-  //     `half` of `src` (LAST: there is none). That of A's last row comes in
-  //     the next step, so this one begins with its own, from `cur`, `own`;
+  // 32 k: the products of the fragments at hand, row by row of A, from set
+  // SET of B's. Between them, one or two at a time and spread evenly (a
+  // product keeps the matrix core for 16 cycles and issues in 4; the LDS
+  // needs 8 for a read of each of four waves: bunched up, the others hold the
+  // products up):
+  //   - the reads of the next fragments, from half `half` of `src` (LAST:
+  //     there are none), A's behind the last use of each, B's into the other
+  //     set or, where there is one, behind the last use. That of A's last row
+  //     comes in the next step, so this one begins with its own, from half
+  //     `own` of `cur`;
   //   - REFILL, the step that changes over to the next stage: after its first
   //     rows every wave is done reading `dst` and its own loads into `src`
   //     have landed, so it syncs there, with products still queued; then the
   //     loads that refill `dst`.
   enum Kind { PLAIN, REFILL, LAST };
-  template <Kind KIND, int PART>
+  template <Kind KIND, int STEP, int PART>
   DEV void step(const TileSrc& s, const lds_char* cur, int own,
                 const lds_char* src, int half, lds_char* dst, int k,
                 f32x4 (&acc)[FM][FN]) {
     constexpr bool FILL = KIND == REFILL;
+    constexpr int SET = STEP % SETS, NEXT = (STEP + 1) % SETS;
     constexpr int ROW0 = !FILL ? 0 : FM > 2 ? 2 : 1;    // first row of reads
-    constexpr int SLOTS = (FM > 2 ? FM - 1 - ROW0 : 1) * FN;
+    constexpr int SLOTS = (FM - ROW0) * FN;
+    // where the loads go: not into a last row that is full of reads
+    constexpr int ROOM = SETS == 2 ? SLOTS : max_(FM - 1 - ROW0, 1) * FN;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        mfma32<T>(acc[i][j], fb[j], fa[i]);
-        if (i == 0 && j == 1) fetch_a(cur, own, FM - 1);
+        mfma32<T>(acc[i][j], fb[SET][j], fa[i]);
+        if (i == 0 && j == 0) fetch_a(cur, own, FM - 1);
         if (KIND != LAST && i >= ROW0) {
+          const int t = (i - ROW0) * FN + j;
           if (j == 1 && i > 0) fetch_a(src, half, i - 1);
           if (j == 3 && i == 2 && ROW0 == 2) fetch_a(src, half, 0);
-          if (i == FM - 1) fetch_b(src, half, j);
+          if (SETS == 1 && i == FM - 1) fetch_b(src, half, 0, j);
+          if (SETS == 2) {
+#pragma unroll
+            for (int b = 0; b < FN; ++b)
+              if (b * SLOTS / FN + 2 == t) fetch_b(src, half, NEXT, b);
+          }
           if (FILL) {
-            const int t = (i - ROW0) * FN + j;
 #pragma unroll
             for (int l = 0; l < LOADS; ++l)
-              if (l * SLOTS / LOADS == t) load<PART>(s, dst, k, l);
+              if (l * ROOM / LOADS == t) load<PART>(s, dst, k, l);
           }
         }
       }
@@ -287,22 +308,22 @@ struct Tile {
     }
     sync();
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fetch_b(even, 0, j);
+    for (int j = 0; j < FN; ++j) fetch_b(even, 0, 0, j);
 #pragma unroll
     for (int i = 0; i < FM - 1; ++i) fetch_a(even, 0, i);
-    int k = s.k_first;
-    if (!SHORT) {
-      // whole turns; a last single stage of one part is left for below
-      for (; k < s.k_last - KODD; k += KTURN) {
-        if (BK == 64) step<PLAIN, 0>(s, even, 0, even, 1, even, 0, acc);
-        step<REFILL, 0>(s, even, LASTH, odd, 0, even, k + KTURN, acc);
-        if (BK == 64) step<PLAIN, 0>(s, odd, 0, odd, 1, odd, 0, acc);
-        step<REFILL, P1>(s, odd, LASTH, even, 0, odd, k + KTURN + KODD, acc);
+    if (SHORT) {
+      if (BK == 64) step<PLAIN, 0, 0>(s, even, 0, even, 1, even, 0, acc);
+      step<LAST, LASTH, 0>(s, even, LASTH, even, 0, even, 0, acc);
+    } else {
+      // turns of two stages: an odd last one is followed by zeros
+      for (int k = s.k_first; k < s.k_last; k += KTURN) {
+        if (BK == 64) step<PLAIN, 0, 0>(s, even, 0, even, 1, even, 0, acc);
+        step<REFILL, LASTH, 0>(s, even, LASTH, odd, 0, even, k + KTURN, acc);
+        if (BK == 64) step<PLAIN, 0, 0>(s, odd, 0, odd, 1, odd, 0, acc);
+        step<REFILL, 1, P1>(s, odd, LASTH, even, 0, odd, k + KTURN + KODD,
+                            acc);
+        mfma_wait();        // behind the loop accumulators may be moved
       }
-    }
-    if (PARTS == 1 && k < s.k_last) {
-      if (BK == 64) step<PLAIN, 0>(s, even, 0, even, 1, even, 0, acc);
-      step<LAST, 0>(s, even, LASTH, even, 0, even, 0, acc);
     }
     // zeros still on their way must not land in what comes after
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
