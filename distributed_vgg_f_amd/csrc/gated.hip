@@ -64,9 +64,18 @@ DEV f32x8 act8(int act, f32x8 g, f32x8& d) {
       d = each(g, [](float v, int) { return v <= 0.f ? 0.f : 1.f; });
       return each(g, [](float v, int) { return v <= 0.f ? 0.f : v; });
     case GELU:
+      // erfc(x) = t (a1 + t (a2 + ... a5)) exp(-x^2), t = 1 / (1 + p x), x >= 0,
+      // off by at most 1.5e-7 (Abramowitz and Stegun, 7.1.26); its
+      // exponential serves the derivative too. erfcf took 10 us more a round
+      // of 256 tiles of 256 x 128.
       return each(g, [&](float v, int r) {
-        float c = 0.5f * erfcf(-0.70710678118654752f * v);
-        d[r] = c + v * 0.39894228040143268f * __expf(-0.5f * v * v);
+        float x = 0.70710678118654752f * __builtin_fabsf(v);
+        float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+        float e = __expf(-x * x);
+        float c = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t *
+                  (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        c = v > 0.f ? 1.f - c : c;
+        d[r] = c + v * 0.39894228040143268f * e;
         return v * c;
       });
     case GELU_TANH:
@@ -101,6 +110,15 @@ DEV u32 keep8(const DropArgs& d, u32 off, i64 i) {
   u32 k = keep4(d, off, i) | keep4(d, off, i + 1) << 4;
   if (sh) k = (k | keep4(d, off, i + 2) << 8) >> sh;
   return k & 255u;
+}
+
+// The same for 4 elements: one block, or two.
+DEV u32 keep4_from(const DropArgs& d, u32 off, i64 i) {
+  const u32 sh = u32(i & 3);
+  i >>= 2;
+  u32 k = keep4(d, off, i);
+  if (sh) k = (k | keep4(d, off, i + 1) << 4) >> sh;
+  return k & 15u;
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -152,19 +170,20 @@ DEV f32x8 widen8(s16x8 v) {
   return o;
 }
 
-// 8 columns of one row, n a multiple of 8: g and u without their biases.
+// 8 columns of a bias from column n, a multiple of 8
+template <class T>
+DEV f32x8 bias8(const u16* b, int n, int N) {
+  f32x8 v{};
+  if (b) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = to_f(b[min(n + r, N - 1)], T());
+  }
+  return v;
+}
+
+// 8 columns of one row of G and U, n a multiple of 8.
 template <class T>
 DEV void finish8(const OutArgs& o, u32 off, int m, int n, f32x8 g, f32x8 u) {
-  if (o.bias[0]) {
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      g[r] += to_f(o.bias[0][min(n + r, o.N - 1)], T());
-  }
-  if (o.bias[1]) {
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      u[r] += to_f(o.bias[1][min(n + r, o.N - 1)], T());
-  }
   if (o.gu) {         // rows of ldg, a multiple of 8, hold all eight
     float* gp = o.gu + (i64)m * o.ldg + n;
     store8f(gp, g);
@@ -200,32 +219,24 @@ struct ProductArgs {
   OutArgs out;          // of FWD
 };
 
-// Eight columns of a row of DGRAD or WGRAD.
-template <class T, int MODE>
-DEV void emit(const ProductArgs& p, int split, int which, int m, int n,
-              f32x8 v) {
-  if (n >= p.cols) return;
-  if (p.splits == 1) {
-    store8((which ? p.c[1] : p.c[0]) + (i64)m * p.cols, n, p.cols,
-           round8<T>(v));
-  } else {
-    constexpr int MATS = MODE == WGRAD ? 2 : 1;
-    store8f(p.slab + (((i64)split * MATS + which) * p.rows + m) * p.slab_ld +
-                n, v);
-  }
-}
-// Eight columns of G and U.
+// Four columns each of two neighbouring fragments, rounded, and traded
+// between the 16-lane rows so that each lane has 8 columns side by side: rows
+// 0 and 2 the first and last 8 of fragment a, rows 1 and 3 those of b.
 template <class T>
-DEV void emit_gated(const ProductArgs& p, int split, u32 off, int m, int n,
-                    f32x8 g, f32x8 u) {
-  if (n >= p.cols) return;
-  if (p.splits == 1) {
-    finish8<T>(p.out, off, m, n, g, u);
-  } else {
-    float* sp = p.slab + ((i64)split * 2 * p.rows + m) * p.slab_ld + n;
-    store8f(sp, g);
-    store8f(sp + (i64)p.rows * p.slab_ld, u);
+DEV s16x8 trade(f32x4 a, f32x4 b) {
+  union { u32 w[4]; s16x4 h[2]; s16x8 v; } t;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    t.h[0][r] = short(from_f(a[r], T()));
+    t.h[1][r] = short(from_f(b[r], T()));
   }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    auto p = __builtin_amdgcn_permlane16_swap(t.w[k], t.w[k + 2], false, false);
+    t.w[k] = p[0];
+    t.w[k + 2] = p[1];
+  }
+  return t.v;
 }
 
 template <class T, int MODE, int FM, int FN, int BK, bool SHORT = false>
@@ -278,53 +289,184 @@ void product_kernel(ProductArgs p) {
   // parts of whole turns: two stages of 64 k, or one of each part
   constexpr int TURN = MODE == DGRAD ? 64 : 128;
   const int turns = (p.k_len + TURN - 1) / TURN;
-  const int q = turns / p.splits, r = turns % p.splits;
-  s.k_first = (split * q + min(split, r)) * TURN;
-  s.k_last = min(s.k_first + (q + (split < r)) * TURN, p.k_len);
+  const int each_ = turns / p.splits, more = turns % p.splits;
+  s.k_first = (split * each_ + min(split, more)) * TURN;
+  s.k_last = min(s.k_first + (each_ + (split < more)) * TURN, p.k_len);
 
   f32x4 acc[FM][FN];
   TL tile;
   tile.run((lds_char*)even, (lds_char*)odd, s, wave, lane, acc);
 
-  // Through LDS, some rows of a wave at a time: the lanes then hold whole
-  // stretches of a row (128 bytes a store and more), and one copy of the
-  // epilogue's code for these rows is enough.
-  constexpr int ROWS = SHORT || BK == 32 ? 16 : 32;
-  constexpr int PITCH = 16 * FN + 4;      // floats; + 4: rows change banks
-  constexpr int MINE = SHORT ? TL::STAGE / 4 : TL::STAGE / 2;
-  static_assert(ROWS * PITCH * 4 <= MINE, "a wave's part of the LDS");
-  float* mine = reinterpret_cast<float*>(
-      SHORT ? even + wave * MINE
-            : (wave & 2 ? odd : even) + (wave & 1) * MINE);
-  __syncthreads();
-  const u32 off = MODE == FWD && p.out.drop ? p.out.d.off() : 0;
+  // Straight from the accumulators: a trip through LDS for wider stores took
+  // 5 us a 256 x 256 tile, of 14 in all besides its products. Lane (c, q):
+  // rows 16 i + c, columns 16 j + 4 q + 0..3 of fragment j, or, traded, the
+  // 8 from column 16 (j + q % 2) + 8 (q / 2) of the fragments j and j + 1.
+  const int c = lane & 15, q = lane >> 4;
+  const int mw = m0 + (wave >> 1) * 16 * FM + c;
+  const int wide = 16 * (q & 1) + 8 * (q >> 1);
+  if constexpr (MODE != FWD) {
+    constexpr int MATS = MODE == WGRAD ? 2 : 1;
+    const int nw = n0 + (wave & 1) * TL::HALF;
 #pragma unroll
-  for (int i = 0; i < FM; i += ROWS / 16) {
+    for (int i = 0; i < FM; ++i) {
+      const int m = mw + 16 * i;
+      if (m >= p.rows) continue;
+      if (p.splits == 1) {
+        u16* o = (which ? p.c[1] : p.c[0]) + (i64)m * p.cols;
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+        for (int j = 0; j < FN; j += 2) {
+          s16x8 v = trade<T>(acc[i][j], acc[i][j + 1]);
+          const int n = nw + 16 * j + wide;
+          if (n < p.cols) store8(o, n, p.cols, v);
+        }
+      } else {
+        float* o = p.slab +
+            (((i64)split * MATS + which) * p.rows + m) * p.slab_ld;
 #pragma unroll
-      for (int q = 0; q < ROWS / 16; ++q)
-        *reinterpret_cast<f32x4*>(mine + (q * 16 + (lane & 15)) * PITCH +
-                                  j * 16 + (lane >> 4) * 4) = acc[i + q][j];
-    // one wave writes and reads: its LDS instructions keep their order
-    const int mw = m0 + (wave >> 1) * 16 * FM + i * 16;
-    if (MODE == FWD) {
-      const int nw = n0 + (wave & 1) * 8 * FN;
-#pragma unroll 1
-      for (int c = lane; c < ROWS * FN; c += 64) {
-        const int m = mw + c / FN, n = c % FN * 8;
-        const float* v = mine + c / FN * PITCH + n;
-        if (m >= p.rows) break;
-        emit_gated<T>(p, split, off, m, nw + n, load8f(v),
-                      load8f(v + 8 * FN));
+        for (int j = 0; j < FN; ++j) {
+          const int n = nw + 16 * j + 4 * q;
+          if (n < p.cols) *reinterpret_cast<f32x4*>(o + n) = acc[i][j];
+        }
       }
-    } else {
-      const int nw = n0 + (wave & 1) * TL::HALF;
-#pragma unroll 2
-      for (int c = lane; c < ROWS * 2 * FN; c += 64) {
-        const int m = mw + c / (2 * FN), n = c % (2 * FN) * 8;
-        f32x8 v = load8f(mine + c / (2 * FN) * PITCH + n);
-        if (m < p.rows) emit<T, MODE>(p, split, which, m, nw + n, v);
+    }
+  } else {
+    constexpr int H = FN / 2;               // fragments of G and of U
+    const int nw = n0 + (wave & 1) * 8 * FN;
+    if (p.splits > 1) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = mw + 16 * i;
+        if (m >= p.rows) continue;
+        float* o = p.slab + ((i64)split * 2 * p.rows + m) * p.slab_ld;
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          const int n = nw + 16 * j + 4 * q;
+          if (n >= p.cols) continue;
+          *reinterpret_cast<f32x4*>(o + n) = acc[i][j];
+          *reinterpret_cast<f32x4*>(o + (i64)p.rows * p.slab_ld + n) =
+              acc[i][j + H];
+        }
+      }
+      return;
+    }
+    const OutArgs& o = p.out;
+    if constexpr (FM == 8) {
+      // Here the straight form spills and runs through ten thousand
+      // instructions once a tile: besides its products a round of tiles took
+      // 16.5 us, through LDS in pieces of 32 rows 14.2, and in this form, 64
+      // rows of a wave at a time, which is all of the LDS, in a loop that has
+      // the next read under way, 12.8. 16-byte chunks trade places by row.
+      static_assert(TL::STAGE == 65536, "32 KB a wave");
+      __syncthreads();
+      float* mine = reinterpret_cast<float*>((wave & 2 ? odd : even) +
+                                             (wave & 1) * 32768);
+      const u32 off = o.drop ? o.d.off() : 0;
+      const int n = nw + (lane & 7) * 8;
+      const f32x8 bg = bias8<T>(o.bias[0], n, o.N);
+      const f32x8 bu = bias8<T>(o.bias[1], n, o.N);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            *reinterpret_cast<f32x4*>(mine + (16 * i + c) * 128 +
+                                      ((4 * j + q) ^ c) * 4) =
+                acc[4 * half + i][j];
+        auto chunk = [&](int row, int k) {
+          return *reinterpret_cast<const f32x4*>(mine + row * 128 +
+                                                 (k ^ (row & 15)) * 4);
+        };
+        f32x4 v[4];
+        auto read = [&](int it) {
+          const int row = (it & 7) * 8 + (lane >> 3), k = (lane & 7) * 2;
+          v[0] = chunk(row, k);
+          v[1] = chunk(row, k + 1);
+          v[2] = chunk(row, k + 16);
+          v[3] = chunk(row, k + 17);
+        };
+        read(0);
+        const int m0w = m0 + (wave >> 1) * 128 + half * 64 + (lane >> 3);
+#pragma unroll 1
+        for (int it = 0; it < 8; ++it) {
+          f32x8 g = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          f32x8 u = __builtin_shufflevector(v[2], v[3], 0, 1, 2, 3, 4, 5, 6, 7);
+          read(it + 1);
+          const int m = m0w + it * 8;
+          if (m < p.rows && n < p.cols)
+            finish8<T>(o, off, m, n, g + bg, u + bu);
+        }
+      }
+      return;
+    }
+    // the mask first, BITS bits a row, in one loop that is not unrolled: one
+    // copy of the generator
+    constexpr int BITS = 4 * H, WORDS = (FM * BITS + 31) / 32;
+    u32 keep[WORDS];
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) keep[w] = 0;
+    if (o.drop) {
+      const u32 off = o.d.off();
+#pragma unroll 1
+      for (int i = 0; i < FM; ++i) {
+        u32 k = 0;
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+          k |= keep4_from(o.d, off, (i64)(mw + 16 * i) * o.N + nw + 16 * j +
+                                        4 * q) << (4 * j);
+#pragma unroll
+        for (int w = 0; w < WORDS - 1; ++w)
+          keep[w] = keep[w] >> BITS | keep[w + 1] << (32 - BITS);
+        keep[WORDS - 1] = keep[WORDS - 1] >> BITS | k << (32 - BITS);
+      }
+    }
+    float bias[2][H][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          bias[h][j][r] = o.bias[h] ? to_f(o.bias[h][min(
+              nw + 16 * j + 4 * q + r, o.N - 1)], T()) : 0.f;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int m = mw + 16 * i;
+      if (m >= p.rows) continue;
+#pragma unroll
+      for (int j = 0; j < H; j += 2) {
+        f32x8 g, u, d;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          g[r] = acc[i][j + r / 4][r % 4] + bias[0][j + r / 4][r % 4];
+          u[r] = acc[i][j + H + r / 4][r % 4] + bias[1][j + r / 4][r % 4];
+        }
+        if (o.gu) {       // rows of ldg, a multiple of 8, hold all four
+          float* gp = o.gu + (i64)m * o.ldg + nw + 16 * j + 4 * q;
+          float* up = gp + (i64)o.M * o.ldg;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (nw + 16 * (j + k) + 4 * q >= p.cols) continue;
+            *reinterpret_cast<f32x4*>(gp + 16 * k) =
+                f32x4{g[4 * k], g[4 * k + 1], g[4 * k + 2], g[4 * k + 3]};
+            *reinterpret_cast<f32x4*>(up + 16 * k) =
+                f32x4{u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]};
+          }
+        }
+        u *= act8(o.act, g, d);
+        if (o.drop) {
+          constexpr int SKIP = 32 * WORDS - FM * BITS;
+          const int at = SKIP + i * BITS + 4 * j;
+          const u32 k = keep[at / 32] >> (at % 32);
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            u[r] = (k >> r & 1) ? u[r] * o.d.scale : 0.f;
+        }
+        s16x8 v = trade<T>(f32x4{u[0], u[1], u[2], u[3]},
+                           f32x4{u[4], u[5], u[6], u[7]});
+        const int n = nw + 16 * j + wide;
+        if (n < p.cols) store8(o.h + (i64)m * o.N, n, o.N, v);
+        __builtin_amdgcn_sched_barrier(0);    // keeps the registers at hand
       }
     }
   }
@@ -368,8 +510,9 @@ __global__ __launch_bounds__(256) void join_gated_kernel(
         }
     }
     if (!in || mine) continue;
-    int m = int(c / per);
-    finish8<T>(o, off, m, int(c - (i64)m * per) * 8, g, u);
+    const int m = int(c / per), n = int(c - (i64)m * per) * 8;
+    finish8<T>(o, off, m, n, g + bias8<T>(o.bias[0], n, o.N),
+               u + bias8<T>(o.bias[1], n, o.N));
   }
 }
 
@@ -525,7 +668,8 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs p) {
       u += load8f(&red[v][1][m][i % 16 * 8]);
     }
     if (p.splits == 1) {
-      finish8<T>(p.out, off, m, n, g, u);
+      finish8<T>(p.out, off, m, n, g + bias8<T>(p.out.bias[0], n, p.N),
+                 u + bias8<T>(p.out.bias[1], n, p.N));
     } else {
       float* sp = p.slab + ((i64)split * 2 * p.M + m) * p.slab_ld + n;
       store8f(sp, g);
