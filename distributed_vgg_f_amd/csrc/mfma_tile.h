@@ -30,10 +30,11 @@ typedef __attribute__((address_space(3))) char lds_char;
 // where it is: through the builtin, result and addend are two registers and
 // the loop around them copies 128 and more of them a turn. In this order the
 // source is the schedule: products and the reads between them stay put.
-// The compiler knows nothing of the instruction's latency here: mfma_wait()
-// ends every piece of straight code with products in it, since the compiler
-// may move accumulators about where pieces join, and mfma_done() comes before
-// any use. tests/test_accumulator_waits.py looks at what was built.
+// The compiler knows nothing of the instruction's timing here: accumulators
+// are set to 0 well before their first product, mfma_wait() ends every piece
+// of straight code with products in it, since the compiler may move
+// accumulators about where pieces join, and mfma_done() comes before any use.
+// tests/test_accumulator_waits.py looks at what was built.
 template <class T>
 DEV void mfma32(f32x4& c, s16x8 a, s16x8 b);
 template <>
@@ -299,7 +300,10 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < FN; ++j) {
+        acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        asm volatile("" : "+a"(acc[i][j]));   // here, not just before its use
+      }
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) load<0>(s, even, s.k_first, l);
     if (!SHORT) {

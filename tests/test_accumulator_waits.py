@@ -2,7 +2,7 @@
 does not know how long their results take. This looks at the code that was
 built: no other instruction touches an accumulator within the 11 wait states
 that v_mfma_f32_16x16x32 needs, on any path, and no vector instruction writes
-an operand of one within the 2 before it."""
+an operand or the accumulator of one within the 4 before it (2 are asked for)."""
 
 import os
 import re
@@ -14,7 +14,7 @@ import pytest
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SO = os.path.join(ROOT, "distributed_vgg_f_amd", "_hipops.so")
 OBJDUMP = shutil.which("llvm-objdump") or "/opt/rocm/llvm/bin/llvm-objdump"
-RESULT, OPERAND = 11, 2
+RESULT, OPERAND = 11, 4
 
 
 def registers(text, bank):
@@ -39,12 +39,13 @@ def too_early(code):
         dst = registers(text.split(",")[0], "a")
         src = registers(",".join(text.split(",")[1:3]), "v")
         gap = 0
-        for _, before, _ in reversed(code[max(0, i - 3):i]):
+        for _, before, _ in reversed(code[max(0, i - OPERAND):i]):
             if gap >= OPERAND:
                 break
-            if before.startswith("v_") and not before.startswith("v_mfma") \
-                    and registers(before.split(",")[0], "v") & src:
-                bad.append((before, text))
+            if before.startswith("v_") and not before.startswith("v_mfma"):
+                to = before.split(",")[0]
+                if registers(to, "v") & src or registers(to, "a") & dst:
+                    bad.append((before, text))
             gap += states(before)
         paths, seen = [(i + 1, 0)], set()
         while paths:
@@ -79,8 +80,10 @@ def test_checker_sees_planted_mistakes():
     assert too_early(jump) == [(mfma, read)]
     write = "v_mov_b32_e32 v5, v9"
     assert too_early([(0, write, None), (8, mfma, None)]) == [(write, mfma)]
-    assert not too_early([(0, write, None), (8, "s_nop 1", None),
+    assert not too_early([(0, write, None), (8, "s_nop 3", None),
                           (16, mfma, None)])
+    zero = "v_accvgpr_write_b32 a1, 0"
+    assert too_early([(0, zero, None), (8, mfma, None)]) == [(zero, mfma)]
 
 
 @pytest.mark.skipif(not (os.path.exists(SO) and os.path.exists(OBJDUMP)),

@@ -241,6 +241,15 @@ def test_long_contractions(M, K, N, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("M,K,N", [(2, 2048, 4096), (33, 4096, 2048),
+                                   (64, 2048, 4096), (129, 4096, 2048),
+                                   (256, 2048, 4096), (2048, 2048, 512)])
+def test_more_tiles_than_the_card_holds(M, K, N):
+    """Several rounds of tiles on every CU, several tiles a CU."""
+    check_case(M, K, N, torch.float16, "gelu", True, p=0.5, seed=M)
+
+
+@gpu
 def test_fused_dropout_is_the_dropout_of_the_result():
     for n in (200, 199):
         ts = [None if t is None else t.to(DEV)
