@@ -36,6 +36,10 @@ class Config:
     #                                    (training-accuracy feature; off for the
     #                                     throughput benchmark)
 
+    fc_gate: str = ""                  # vggf / vgg16: activation of gated fc6/fc7
+    #                                    (silu, gelu, gelu_tanh, relu, sigmoid);
+    #                                    empty = linear + ReLU
+
     # training
     batch_size: int = 256              # per-GPU
     lr: float = 0.01

@@ -49,6 +49,45 @@ class Linear(nn.Module):
         return ops.linear(x, self.weight, self.bias, self.relu)
 
 
+class GatedLinear(nn.Module):
+    """act(x @ w_gate + b_gate) * (x @ w_up + b_up), x [M,K], both w [K,N].
+
+    With a Dropout layer as second argument its mask is drawn in the same
+    kernel (the layer's counter advances as if it had been called)."""
+
+    def __init__(self, k: int, n: int, act: str = "silu", bias: bool = True,
+                 std: Optional[float] = None):
+        super().__init__()
+        if act not in ops.ACTIVATIONS:
+            raise ValueError(f"unknown activation {act!r}; have "
+                             f"{list(ops.ACTIVATIONS)}")
+        self.act = act
+        std = std if std is not None else math.sqrt(2.0 / k)
+        self.weight_gate = nn.Parameter(torch.randn(k, n) * std)
+        self.weight_up = nn.Parameter(torch.randn(k, n) * std)
+        self.bias_gate = nn.Parameter(torch.zeros(n)) if bias else None
+        self.bias_up = nn.Parameter(torch.zeros(n)) if bias else None
+
+    def forward(self, x, drop: Optional["Dropout"] = None):
+        w = (self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
+        if drop is None or not drop.training or drop.p <= 0.0:
+            return ops.gated_linear(x, *w, act=self.act)
+        drop._calls += 1
+        return ops.gated_linear(x, *w, act=self.act, p=drop.p, seed=drop.seed,
+                                offset=drop._calls)
+
+
+def hidden_fc(k: int, n: int, gate: str = "") -> nn.Module:
+    """A hidden layer of a classifier's head: linear and ReLU, or the gated
+    unit with the activation that `gate` names."""
+    return GatedLinear(k, n, gate) if gate else Linear(k, n, relu=True)
+
+
+def run_hidden(fc: nn.Module, drop: "Dropout", x):
+    """A hidden layer and the dropout behind it."""
+    return fc(x, drop) if isinstance(fc, GatedLinear) else drop(fc(x))
+
+
 class LRN(nn.Module):
     def __init__(self, size: int = 5, alpha: float = 1e-4, beta: float = 0.75,
                  k: float = 2.0):

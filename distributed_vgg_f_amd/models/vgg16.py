@@ -11,7 +11,8 @@ import torch
 import torch.nn as nn
 
 from ..config import Config
-from .layers import Conv2d, Dropout, Linear, MaxPool
+from .layers import (Conv2d, Dropout, Linear, MaxPool, hidden_fc,
+                     run_hidden)
 
 
 _CFG_D = [64, 64, "M", 128, 128, "M", 256, 256, 256, "M",
@@ -33,15 +34,15 @@ class VGG16(nn.Module):
         with torch.no_grad():
             probe = torch.zeros(1, cfg.image_size, cfg.image_size, cfg.channels)
             flat = self.features(probe).numel()     # 512*7*7 = 25088 at 224
-        self.fc6 = Linear(flat, 4096, relu=True)
+        self.fc6 = hidden_fc(flat, 4096, cfg.fc_gate)
         self.drop6 = Dropout(cfg.dropout, cfg.seed)
-        self.fc7 = Linear(4096, 4096, relu=True)
+        self.fc7 = hidden_fc(4096, 4096, cfg.fc_gate)
         self.drop7 = Dropout(cfg.dropout, cfg.seed + 1)
         self.fc8 = Linear(4096, cfg.num_classes, relu=False, std=0.01)
 
     def forward(self, x):
         x = self.features(x)
         x = x.reshape(x.shape[0], -1)
-        x = self.drop6(self.fc6(x))
-        x = self.drop7(self.fc7(x))
+        x = run_hidden(self.fc6, self.drop6, x)
+        x = run_hidden(self.fc7, self.drop7, x)
         return self.fc8(x)

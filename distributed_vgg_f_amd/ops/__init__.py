@@ -15,7 +15,8 @@ from . import cpu_ref
 from . import native  # noqa: F401  (re-export for engine / tests)
 
 
-_ACT_ID = {name: i for i, name in enumerate(cpu_ref.ACTIVATIONS)}
+ACTIVATIONS = tuple(cpu_ref.ACTIVATIONS)      # of gated_linear
+_ACT_ID = {name: i for i, name in enumerate(ACTIVATIONS)}
 
 
 def conv2d(x, w, bias=None, stride: int = 1, pad: int = 0, relu: bool = False):
@@ -46,9 +47,9 @@ def gated_linear(x, w_gate, w_up, bias_gate=None, bias_up=None,
     and strides; sums in 32 bits. Operands whose rows do not start on 16
     bytes are copied to rows that do, once a call. Differentiates once.
     """
-    if act not in cpu_ref.ACTIVATIONS:
+    if act not in _ACT_ID:
         raise ValueError(f"gated_linear: unknown activation {act!r}; have "
-                         f"{list(cpu_ref.ACTIVATIONS)}")
+                         f"{list(ACTIVATIONS)}")
     if not p <= 1.0:
         raise ValueError(f"gated_linear: p must not be above 1, got {p}")
     if not x.is_cuda or p == 1.0:
