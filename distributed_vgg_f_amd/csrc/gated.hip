@@ -143,15 +143,30 @@ DEV void store8f(float* p, f32x8 v) {
   *reinterpret_cast<f32x4*>(p + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
 }
 
-// 8 columns to row c of N
+// 8 columns to row c of N. Rows of odd lengths start anywhere: those stores
+// are as wide as the compiler makes them for 2-byte alignment.
 DEV void store8(u16* c, int n, int N, s16x8 v) {
   if ((N & 7) == 0) {
     *reinterpret_cast<s16x8*>(c + n) = v;
+  } else if (n + 8 <= N) {
+    __builtin_memcpy(c + n, &v, 16);
   } else {
 #pragma unroll
     for (int r = 0; r < 8; ++r)
       if (n + r < N) c[n + r] = u16(v[r]);
   }
+}
+// 8 columns of a row of N, zeros behind it
+DEV s16x8 load8(const u16* c, int n, int N) {
+  s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (n + 8 <= N) {
+    __builtin_memcpy(&v, c + n, 16);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (n + r < N) v[r] = short(c[n + r]);
+  }
+  return v;
 }
 
 template <class T>
@@ -240,7 +255,7 @@ DEV s16x8 trade(f32x4 a, f32x4 b) {
 }
 
 template <class T, int MODE, int FM, int FN, int BK, bool SHORT = false>
-__global__ __launch_bounds__(256, SHORT || BK == 32 ? 4 : FM == 8 ? 1 : 2)
+__global__ __launch_bounds__(256, SHORT || BK == 32 ? 4 : FM * FN == 64 ? 1 : 2)
 void product_kernel(ProductArgs p) {
   constexpr bool ATR = MODE == WGRAD, BTR = MODE != DGRAD;
   using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN, BK,
@@ -350,7 +365,7 @@ void product_kernel(ProductArgs p) {
       return;
     }
     const OutArgs& o = p.out;
-    if constexpr (FM == 8) {
+    if constexpr (FM * FN == 64) {
       // Here the straight form spills and runs through ten thousand
       // instructions once a tile: besides its products a round of tiles took
       // 16.5 us, through LDS in pieces of 32 rows 14.2, and in this form, 64
@@ -545,7 +560,8 @@ __global__ __launch_bounds__(256) void join_plain_kernel(
 // lane (c, q) holds column 8 c + j and its 8 k: what the matrix instruction
 // takes. The next 32 k are on their way meanwhile (32 KB a wave). The four
 // waves of a block, each with its part of the contraction, meet in LDS; parts
-// of several blocks meet in join_gated_kernel.
+// of several blocks meet in join_gated_kernel. (With the fragments of 32 or 64
+// rows the tiles are faster: 64 x 25088 x 4096 in 91 us, this way in 112.)
 struct RowsArgs {
   const u16* x;
   const u16* w[2];
@@ -578,7 +594,7 @@ DEV f32x4 mfma_of(s16x8 a, s16x8 b, f32x4 c, _Float16) {
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void rows_kernel(RowsArgs p) {
+__global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs p) {
   __shared__ __attribute__((aligned(16))) float red[4][2][16][128];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wave = uniform(threadIdx.x >> 6);
@@ -648,33 +664,29 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs p) {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float* d = &red[wave][h][c][(4 * q + r) * 8];
         f32x8 v;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = acc[h][j][r];
-        store8f(d, v);
+        store8f(&red[wave][h][c][(4 * q + r) * 8], v);
       }
   }
   __syncthreads();
   const u32 off = p.out.drop ? p.out.d.off() : 0;
-  for (int i = threadIdx.x; i < p.M * 16; i += 256) {
-    const int m = i / 16, n = n0 + i % 16 * 8;
-    if (n >= p.N) continue;
-    f32x8 g = load8f(&red[0][0][m][i % 16 * 8]);
-    f32x8 u = load8f(&red[0][1][m][i % 16 * 8]);
+  const int m = threadIdx.x / 16, k = threadIdx.x % 16 * 8, n = n0 + k;
+  if (m >= p.M || n >= p.N) return;
+  f32x8 g = load8f(&red[0][0][m][k]), u = load8f(&red[0][1][m][k]);
 #pragma unroll
-    for (int v = 1; v < 4; ++v) {
-      g += load8f(&red[v][0][m][i % 16 * 8]);
-      u += load8f(&red[v][1][m][i % 16 * 8]);
-    }
-    if (p.splits == 1) {
-      finish8<T>(p.out, off, m, n, g + bias8<T>(p.out.bias[0], n, p.N),
-                 u + bias8<T>(p.out.bias[1], n, p.N));
-    } else {
-      float* sp = p.slab + ((i64)split * 2 * p.M + m) * p.slab_ld + n;
-      store8f(sp, g);
-      store8f(sp + (i64)p.M * p.slab_ld, u);
-    }
+  for (int v = 1; v < 4; ++v) {
+    g += load8f(&red[v][0][m][k]);
+    u += load8f(&red[v][1][m][k]);
+  }
+  if (p.splits == 1) {
+    finish8<T>(p.out, off, m, n, g + bias8<T>(p.out.bias[0], n, p.N),
+               u + bias8<T>(p.out.bias[1], n, p.N));
+  } else {
+    float* sp = p.slab + ((i64)split * 2 * p.M + m) * p.slab_ld + n;
+    store8f(sp, g);
+    store8f(sp + (i64)p.M * p.slab_ld, u);
   }
 }
 
@@ -710,15 +722,9 @@ __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
     for (int m = r0 + ty; m < r1; m += 8) {
       const float* gp = a.gu + (i64)m * a.ldg + n;
       f32x8 g = load8f(gp), u = load8f(gp + (i64)a.M * a.ldg);
-      s16x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
-      const u16* hp = a.dh + (i64)m * a.ldh + n;
-      if (wide) {
-        h = *reinterpret_cast<const s16x8*>(hp);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (n + j < a.N) h[j] = short(hp[j]);
-      }
+      const u16* hp = a.dh + (i64)m * a.ldh;
+      s16x8 h = wide ? *reinterpret_cast<const s16x8*>(hp + n)
+                     : load8(hp, n, a.N);
       u32 keep = 255u;
       if (a.drop) {
         i64 i = (i64)m * a.N + n;
@@ -787,20 +793,32 @@ __global__ __launch_bounds__(256) void bias_join_kernel(
 
 // -------------------------------------------------------------- rows apart
 // Copies rows of any length and alignment to rows of whole vectors, zeros
-// behind them: what the tiles cannot load goes through here once a call.
-__global__ __launch_bounds__(256) void pad_rows_kernel(
-    const u16* __restrict__ in, i64 sr, i64 sc, u16* __restrict__ out,
-    i64 rows, int cols, int ld) {
-  const int per = ld / 8;
-  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < rows * per;
+// behind them: what the tiles cannot load goes through here once a call, all
+// operands in one launch.
+struct PadArgs {
+  const u16* in[3];
+  u16* out[3];
+  i64 sr[3], sc[3], rows[3];
+  int cols[3], ld[3];
+};
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
+  const int t = blockIdx.y;
+  const int per = a.ld[t] / 8, cols = a.cols[t];
+  const i64 sc = a.sc[t];
+  for (i64 c = (i64)blockIdx.x * 256 + threadIdx.x; c < a.rows[t] * per;
        c += (i64)gridDim.x * 256) {
-    i64 r = c / per;
-    int n = int(c - r * per) * 8;
+    const i64 r = c / per;
+    const int n = int(c - r * per) * 8;
+    const u16* in = a.in[t] + r * a.sr[t];
     s16x8 v;
+    if (sc == 1) {
+      v = load8(in, n, cols);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = n + j < cols ? short(in[r * sr + (n + j) * sc]) : short(0);
-    *reinterpret_cast<s16x8*>(out + c * 8) = v;
+      for (int j = 0; j < 8; ++j)
+        v[j] = n + j < cols ? short(in[(n + j) * sc]) : short(0);
+    }
+    *reinterpret_cast<s16x8*>(a.out[t] + c * 8) = v;
   }
 }
 
@@ -816,21 +834,35 @@ static u16* mptr(const at::Tensor& t) {
 
 // A matrix that the tiles can load: unit column stride, rows that start on
 // 16 bytes and whose last vector may be read whole.
-static at::Tensor loadable(const at::Tensor& t) {
-  i64 rows = t.size(0), cols = t.size(1);
-  bool ok = t.stride(1) == 1 && cols % 8 == 0 &&
-            (rows == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= cols)) &&
-            reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  if (ok) return t;
-  auto out = at::empty({rows, up(cols, 8)}, t.options());
-  i64 chunks = out.numel() / 8;
-  if (chunks)
-    hipLaunchKernelGGL(pad_rows_kernel,
-                       dim3(u32(std::min<i64>((chunks + 255) / 256, 8192))),
-                       dim3(256), 0, cur_stream(), cptr(t), t.stride(0),
-                       t.stride(1), mptr(out), rows, int(cols),
-                       int(out.size(1)));
-  return out;
+static bool loadable(const at::Tensor& t) {
+  return t.stride(1) == 1 && t.size(1) % 8 == 0 &&
+         (t.size(0) == 1 ||
+          (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+// Makes all of them loadable, copies of those that are not.
+static void make_loadable(at::Tensor (&t)[3]) {
+  PadArgs a{};
+  i64 most = 0;
+  int n = 0;
+  for (auto& m : t) {
+    if (loadable(m)) continue;
+    auto out = at::empty({m.size(0), up(m.size(1), 8)}, m.options());
+    a.in[n] = cptr(m);
+    a.out[n] = mptr(out);
+    a.sr[n] = m.stride(0);
+    a.sc[n] = m.stride(1);
+    a.rows[n] = m.size(0);
+    a.cols[n] = int(m.size(1));
+    a.ld[n] = int(out.size(1));
+    most = std::max<i64>(most, out.numel() / 8);
+    ++n;
+    m = out;
+  }
+  if (!most) return;
+  dim3 grid(u32(std::min<i64>((most + 255) / 256, 8192)), n);
+  hipLaunchKernelGGL(pad_rows_kernel, grid, dim3(256), 0, cur_stream(), a);
+  HIP_CHECK(hipGetLastError());
 }
 // a single row may carry any stride
 static i64 ld_of(const at::Tensor& t) {
@@ -1076,8 +1108,9 @@ std::vector<at::Tensor> gated_fwd(
                        d.offset_ptr,
                        reinterpret_cast<i64*>(used.data_ptr<int64_t>()));
   }
-  auto xl = loadable(x), gl = loadable(wg);
-  auto ul = loadable(wu);
+  at::Tensor ops_[3] = {x, wg, wu};
+  make_loadable(ops_);
+  at::Tensor &xl = ops_[0], &gl = ops_[1], &ul = ops_[2];
   if (ld_of(ul) != ld_of(gl)) {           // one pitch for both
     gl = gl.contiguous();
     ul = ul.contiguous();
