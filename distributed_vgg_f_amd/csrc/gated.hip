@@ -691,15 +691,19 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(RowsArgs p) {
 }
 
 // ------------------------------------------- between dH and the products
-// dG and dU (rows of ldg, zeros behind N) and, if `part` is given, the sums
-// of each block's rows: part [gridDim.y][2][ldg]. A thread takes 8 columns,
-// a block 256, its 8 groups of 32 threads every eighth row.
+// dG and dU (rows of ldg, zeros behind N) and, where biases want them, their
+// column sums: of each block's rows as part [gridDim.y][2][ldg], or, if one
+// block takes all rows, the gradients themselves. A thread takes 8 columns, a
+// block CB, its groups of CB / 8 threads every (2048 / CB)th row. CB = 64 for
+// up to 64 rows: the sums then need no second kernel (64 x 4096: 6.3 us in
+// place of 9.5; 256 x 4096: 14.3 and 9.5).
 struct MidArgs {
   const u16* dh;
   i64 ldh;
   const float* gu;
   u16* dgu;
   float* part;
+  u16* db[2];
   int M, N;
   i64 ldg;
   int rows_per_block;
@@ -707,11 +711,12 @@ struct MidArgs {
   DropArgs d;
 };
 
-template <class T>
+template <class T, int CB>
 __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
-  __shared__ float red[8][2][256];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int n = blockIdx.x * 256 + tx * 8;
+  constexpr int GROUPS = 2048 / CB;
+  __shared__ float red[GROUPS][2][CB];
+  const int tx = threadIdx.x % (CB / 8), ty = threadIdx.x / (CB / 8);
+  const int n = blockIdx.x * CB + tx * 8;
   const u32 off = a.drop ? a.d.off() : 0;
   f32x8 sg{}, su{};
   const int r0 = blockIdx.y * a.rows_per_block;
@@ -719,7 +724,7 @@ __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
   const bool wide = (a.N & 7) == 0 && (a.ldh & 7) == 0 &&
                     (reinterpret_cast<uintptr_t>(a.dh) & 15) == 0;
   if (n < a.ldg) {
-    for (int m = r0 + ty; m < r1; m += 8) {
+    for (int m = r0 + ty; m < r1; m += GROUPS) {
       const float* gp = a.gu + (i64)m * a.ldg + n;
       f32x8 g = load8f(gp), u = load8f(gp + (i64)a.M * a.ldg);
       const u16* hp = a.dh + (i64)m * a.ldh;
@@ -747,24 +752,21 @@ __global__ __launch_bounds__(256) void mid_kernel(MidArgs a) {
       *reinterpret_cast<s16x8*>(op + (i64)a.M * a.ldg) = ou;
     }
   }
-  if (!a.part) return;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    red[ty][0][tx * 8 + j] = sg[j];
-    red[ty][1][tx * 8 + j] = su[j];
-  }
+  if (!a.part && !a.db[0] && !a.db[1]) return;
+  store8f(&red[ty][0][tx * 8], sg);
+  store8f(&red[ty][1][tx * 8], su);
   __syncthreads();
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.ldg) return;
-  float vg = 0.f, vu = 0.f;
+  for (int i = threadIdx.x; i < 2 * CB; i += 256) {
+    const int h = i / CB, c = blockIdx.x * CB + i % CB;
+    float v = 0.f;
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    vg += red[r][0][threadIdx.x];
-    vu += red[r][1][threadIdx.x];
+    for (int r = 0; r < GROUPS; ++r) v += red[r][h][i % CB];
+    if (a.part) {
+      if (c < a.ldg) a.part[((i64)blockIdx.y * 2 + h) * a.ldg + c] = v;
+    } else if (c < a.N && a.db[h]) {
+      a.db[h][c] = from_f(v, T());
+    }
   }
-  float* pp = a.part + (i64)blockIdx.y * 2 * a.ldg + c;
-  pp[0] = vg;
-  pp[a.ldg] = vu;
 }
 
 // 32 columns a block, 8 groups of threads a part of the blocks' sums each.
@@ -1191,32 +1193,30 @@ std::vector<at::Tensor> gated_bwd(
     a.act = int(act);
     a.drop = p > 0.0;
     a.d = d;
-    const int bx = ceil_div(ldg, 256);
+    const bool half = type == at::kHalf, one = M <= 64;
+    const int bx = ceil_div(ldg, one ? 64 : 256);
     // about 2048 blocks; 8 rows a turn
-    a.rows_per_block = int(std::max<i64>(8, up(ceil_div(M * bx, 2048), 8)));
+    a.rows_per_block =
+        one ? int(M) : int(std::max<i64>(8, up(ceil_div(M * bx, 2048), 8)));
     const int by = ceil_div(M, a.rows_per_block);
+    TORCH_CHECK(by < 65536, "gated_linear: too many rows");
     at::Tensor part;
-    if (bias) {
+    if (bias && one) {
+      a.db[0] = ptr(3);
+      a.db[1] = ptr(4);
+    } else if (bias) {
       part = at::empty({by, 2, ldg}, opt.dtype(at::kFloat));
       a.part = part.data_ptr<float>();
     }
-    const bool half = type == at::kHalf;
     auto st = cur_stream();
-    TORCH_CHECK(by < 65536, "gated_linear: too many rows");
-    if (half)
-      hipLaunchKernelGGL(mid_kernel<_Float16>, dim3(bx, by), dim3(256), 0, st,
-                         a);
-    else
-      hipLaunchKernelGGL(mid_kernel<__bf16>, dim3(bx, by), dim3(256), 0, st,
-                         a);
-    if (bias) {
-      dim3 g(ceil_div(N, 32), 2);
-      if (half)
-        hipLaunchKernelGGL(bias_join_kernel<_Float16>, g, dim3(256), 0, st,
-                           a.part, by, int(N), ldg, ptr(3), ptr(4));
-      else
-        hipLaunchKernelGGL(bias_join_kernel<__bf16>, g, dim3(256), 0, st,
-                           a.part, by, int(N), ldg, ptr(3), ptr(4));
+    auto mid = one ? (half ? mid_kernel<_Float16, 64> : mid_kernel<__bf16, 64>)
+                   : (half ? mid_kernel<_Float16, 256>
+                           : mid_kernel<__bf16, 256>);
+    hipLaunchKernelGGL(mid, dim3(bx, by), dim3(256), 0, st, a);
+    if (a.part) {
+      auto join = half ? bias_join_kernel<_Float16> : bias_join_kernel<__bf16>;
+      hipLaunchKernelGGL(join, dim3(ceil_div(N, 32), 2), dim3(256), 0, st,
+                         a.part, by, int(N), ldg, ptr(3), ptr(4));
     }
     HIP_CHECK(hipGetLastError());
     const u16* dg = cptr(dgu);
