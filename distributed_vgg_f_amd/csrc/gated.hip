@@ -876,9 +876,10 @@ constexpr int ROWS_MAX = 16, ROWS_TARGET = 256;
 struct Plan { int fm, fn, bk, splits, tiles_m, tiles_n; bool brief; };
 
 // Which tile, and into how many parts the contraction is split: the least
-// time by a model of what the tiles measured over 44 products from 1 x 512 to
-// 8192 x 8192 rows and columns (it is off by 13 % there; what it picks is 2 %
-// slower than the best of all tiles and splits in the mean, 17 % at worst).
+// time by a model of what the tiles measured over the 138 products of 46
+// shapes of 17 to 8192 rows and 64 to 25088 columns (it is off by 16 % there;
+// what it picks is 2 % slower than the best of all tiles and splits in the
+// mean, 20 % at worst).
 // Microseconds. A stage costs `one` if a tile has its CU to itself and `all`
 // if the CU is full; `edge` is a tile's first loads and its epilogue.
 static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
@@ -888,7 +889,8 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
                                {2, 4, 64, 3, 0.61, 0.93, 2.8, false},
                                {4, 4, 32, 4, 0.69, 1.85, 4.0, false},
                                {4, 4, 64, 4, 0.69, 1.85, 3.9, true}};
-  constexpr double CUS = 256, MEM = 4.5e6, JOIN = 2.8, JOIN_MEM = 7e6;
+  constexpr double CUS = 256, MEM = 4.5e6, JOIN_MEM = 7e6;
+  const double join = mode == FWD ? 4.0 : 2.4;
   // turns of the loop, and stages in each
   const int turns = ceil_div(k_len, mode == DGRAD ? 64 : 128);
   const double mats = mode == DGRAD ? 1 : 2;
@@ -921,7 +923,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
       const double full = std::floor(wgs / slots);
       double t = full * round(slots) + round(wgs - full * slots);
       t = std::sqrt(std::sqrt(t * t * t * t + mem * mem * mem * mem));
-      if (sp > 1) t += JOIN + sp * mats * out * 8 / JOIN_MEM;
+      if (sp > 1) t += join + sp * mats * out * 8 / JOIN_MEM;
       if (least == 0 || t < least) {
         least = t;
         best = Plan{k.fm, k.fn, k.bk, sp, tm, tn, k.brief};
