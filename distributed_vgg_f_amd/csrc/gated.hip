@@ -1172,13 +1172,22 @@ std::vector<at::Tensor> gated_bwd(
       TORCH_CHECK(out->is_contiguous() && out->device() == x.device() &&
                   out->numel() == shapes[i][0] * shapes[i][1],
                   "gated_linear: bad gradient buffer");
-    // a buffer of another type is filled by a copy at the end
-    bool direct = out && out->scalar_type() == type;
+    // a buffer of another type, or one that vectors do not fit, is filled by
+    // a copy at the end
+    bool direct = out && out->scalar_type() == type &&
+                  reinterpret_cast<uintptr_t>(out->data_ptr()) % 16 == 0;
     grads[i] = direct ? *out
                       : at::empty({shapes[i][0], shapes[i][1]}, opt);
     result[i] = out ? *out : i < 3 ? grads[i] : grads[i].view({N});
   }
-  auto ptr = [&](int i) { return grads[i].defined() ? mptr(grads[i]) : nullptr; };
+  for (int i = 1; i < 5; i += 2)
+    TORCH_CHECK(!result[i].defined() || !result[i + 1].defined() ||
+                !outs[i] || !outs[i + 1] ||
+                outs[i]->data_ptr() != outs[i + 1]->data_ptr(),
+                "gated_linear: gate and up share one gradient buffer");
+  auto ptr = [&](int i) {
+    return grads[i].defined() ? mptr(grads[i]) : nullptr;
+  };
   if (M == 0) {
     for (auto& g : grads) if (g.defined()) g.zero_();
   } else {
@@ -1256,7 +1265,7 @@ std::vector<at::Tensor> gated_bwd(
     }
   }
   for (int i = 0; i < 5; ++i)
-    if (result[i].defined() && result[i].scalar_type() != type)
+    if (result[i].defined() && result[i].data_ptr() != grads[i].data_ptr())
       result[i].view(-1).copy_(grads[i].view(-1));
   return result;
 }

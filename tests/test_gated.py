@@ -327,6 +327,91 @@ def test_one_gradient_alone(which):
 
 
 @gpu
+def test_one_weight_twice():
+    x, w, _, b, _, dh = [t.to(DEV) for t in
+                         make(33, 40, 48, torch.float16, True)]
+    w, b = w.requires_grad_(), b.requires_grad_()
+    h = ops.gated_linear(x, w, w, b, b)
+    dw, db = torch.autograd.grad(h, (w, b), dh)
+    two = [t.detach().clone().requires_grad_() for t in (w, w, b, b)]
+    parts = torch.autograd.grad(ops.gated_linear(x, *two), two, dh)
+    assert torch.equal(dw, parts[0] + parts[1])
+    assert torch.equal(db, parts[2] + parts[3])
+
+
+@gpu
+def test_one_buffer_for_two_gradients_is_refused():
+    x, w, _, b, _, dh = [t.to(DEV) for t in
+                         make(8, 40, 48, torch.bfloat16, True)]
+    w = w.requires_grad_()
+    w._dvgg_gbuf = torch.zeros_like(w)
+    h = ops.gated_linear(x, w, w)
+    with pytest.raises(RuntimeError, match="share one gradient buffer"):
+        h.backward(dh)
+
+
+@gpu
+def test_gradient_buffer_anywhere_in_memory():
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in
+                             make(20, 40, 48, torch.bfloat16, True)]
+    want = run_all([x, wg, wu, bg, bu, dh], "silu")[2:]
+    leaves = [t.detach().requires_grad_() for t in (wg, wu, bg, bu)]
+    room = [torch.zeros(t.numel() + 3, dtype=t.dtype, device=DEV)
+            for t in leaves]
+    for t, r in zip(leaves, room):
+        t._dvgg_gbuf = r[3:].view(t.shape)
+    ops.gated_linear(x, *leaves).backward(dh)
+    for name, t, w in zip(NAMES[2:], leaves, want):
+        assert torch.equal(t._dvgg_gbuf, w), name
+        assert torch.equal(t.grad, w), name
+
+
+@gpu
+def test_broadcast_input_and_inference_mode():
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in
+                             make(1, 40, 48, torch.float16, True)]
+    row = x.detach().requires_grad_()
+    h = ops.gated_linear(row.expand(30, 40), wg, wu, bg, bu)
+    g, = torch.autograd.grad(h, row, dh.expand(30, 48))
+    full = x.expand(30, 40).contiguous().requires_grad_()
+    h2 = ops.gated_linear(full, wg, wu, bg, bu)
+    g2, = torch.autograd.grad(h2, full, dh.expand(30, 48).contiguous())
+    assert torch.equal(h, h2)
+    assert torch.equal(g, g2.sum(0, keepdim=True))
+    with torch.inference_mode():
+        assert torch.equal(ops.gated_linear(full, wg, wu, bg, bu), h2)
+
+
+@gpu
+def test_changed_input_is_noticed():
+    x, wg, wu, *_ = [None if t is None else t.to(DEV)
+                     for t in make(20, 40, 48, torch.float16, False)]
+    wg.requires_grad_()
+    h = ops.gated_linear(x, wg, wu)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        h.sum().backward()
+
+
+@gpu
+def test_two_streams_at_once():
+    sets = [make(70, 2056, 136, torch.bfloat16, True, seed=s)
+            for s in range(2)]
+    want = [run_all(ts, "silu", 0.5, 7, 3) for ts in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = run_all(sets[i], "silu", 0.5, 7, 3)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for name, p, q in zip(NAMES, a, b):
+            assert torch.equal(p, q), name
+
+
+@gpu
 def test_rows_of_infinities_stay_apart():
     x, wg, wu, *_ = [None if t is None else t.to(DEV)
                      for t in make(40, 64, 72, torch.bfloat16, False)]
