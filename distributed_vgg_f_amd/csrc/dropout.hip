@@ -1,5 +1,13 @@
 // Dropout without a stored mask (K12): y = keep * x / (1 - p), the same
 // kernel forwards on x and backwards on dy.
+//
+// Bound by memory, one read and one write of each element: forward and
+// backward over 47.8M bf16 take 78 us (4.9 TB/s), over 268M fp16 440 us (4.88);
+// a large copy reaches 5.12. A stored mask would add a byte to the 4 of each
+// element and direction. The generator needs 20 64-bit products, a quarter of
+// the rate, for a block of four elements: by count 60 % of that time, behind
+// the loads. Below a few million elements the host's launches are the bound
+// (256 x 4096: 27 us for two kernels of 3).
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>

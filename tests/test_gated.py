@@ -327,6 +327,46 @@ def test_one_gradient_alone(which):
 
 
 @gpu
+def test_results_past_32_bits():
+    # 2^31 results and more; only the last rows have gradients: the terms of
+    # the others are zeros and add no error
+    M, K, N, last = (1 << 22) + 5, 8, 520, 37
+    ts = make(last, K, N, torch.bfloat16, True)
+    outs, errs = oracle(*ts, "silu", 1.0)
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in ts]
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    big = torch.randn(M, K, generator=gen, device=DEV).bfloat16()
+    big[-last:] = x
+    with torch.no_grad():
+        plain = ops.gated_linear(big, wg, wu, bg, bu)
+        h = ops.gated_linear(big, wg, wu, bg, bu, p=0.5, seed=9, offset=2)
+        # doubling is exact
+        assert torch.equal(h, ops.dropout(plain, 0.5, 9, 2))
+    del h, plain
+    leaves = [t.requires_grad_() for t in (big, wg, wu, bg, bu)]
+    zero = torch.zeros(M, N, dtype=x.dtype, device=DEV)
+    zero[-last:] = dh
+    h = ops.gated_linear(*leaves)
+    got = torch.autograd.grad(h, leaves, zero)
+    assert not bool(got[0][:-last].any())
+    compare([h[-last:], got[0][-last:], *got[1:]], outs, errs, x.dtype)
+
+
+@gpu
+def test_rows_far_apart():
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in
+                             make(20, 40, 48, torch.float16, True)]
+    want = run_all([x, wg, wu, bg, bu, dh], "silu")
+    far = torch.empty(20, (1 << 21) + 8, dtype=x.dtype, device=DEV)
+    far[:, :40] = x
+    wide = torch.empty(40, (1 << 21) + 8, dtype=x.dtype, device=DEV)
+    wide[:, :48] = wg
+    got = run_all([far[:, :40], wide[:, :48], wu, bg, bu, dh], "silu")
+    for name, a, b in zip(NAMES, got, want):
+        assert torch.equal(a, b), name
+
+
+@gpu
 def test_one_weight_twice():
     x, w, _, b, _, dh = [t.to(DEV) for t in
                          make(33, 40, 48, torch.float16, True)]
