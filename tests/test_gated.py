@@ -581,6 +581,31 @@ def test_replayed_graph_and_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("K,N", [(2056, 136), (2055, 133)])
+def test_two_graphs_in_turn(K, N):
+    # answers of few and of more rows, each split and joined, in two graphs
+    # whose replays alternate
+    sets = [[t.to(DEV) for t in make(M, K, N, torch.float16, True)[:5]]
+            for M in (4, 40)]
+    graphs, got = [], []
+    for ts in sets:
+        ops.gated_linear(*ts, act="gelu")
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(ops.gated_linear(*ts, act="gelu"))
+    for replay in range(4):
+        for i, ts in enumerate(sets):
+            ts[0].copy_(make(ts[0].shape[0], K, N, torch.float16, True,
+                             seed=replay)[0])
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for h, ts in zip(got, sets):
+            assert torch.equal(h, ops.gated_linear(*ts, act="gelu")), replay
+
+
+@gpu
 def test_offset_counted_up_before_backward():
     ts = make(20, 64, 72, torch.bfloat16, True)
     *leaves, dh = [t.to(DEV) for t in ts]
