@@ -260,8 +260,10 @@ DEV s16x8 trade(f32x4 a, f32x4 b) {
 // tiles with the matrix cores busy for 70 % of the cycles. What bounds it
 // there is power: the more of them are busy, the lower the clock (1.75 GHz),
 // and 32x32x16 products took 917 and 970 us in place of 840 and 876. At 256 x
-// 9216 x 4096 the forward product (63 us, joined in 11) waits for memory: 151
-// MB of weights at 2.4 TB/s, as much in flight as LDS holds.
+// 9216 x 4096 the forward product (63 us, joined in 11) moves 151 MB of
+// weights and 34 of slabs; by count its tiles of 128 x 128 keep LDS busy for
+// two thirds of that time. A ring of four stages of 32 k, half as much again
+// in flight, came within 4 % either way over 26 shapes: latency is not the bound.
 template <class T, int MODE, int FM, int FN, int BK, bool SHORT = false>
 __global__ __launch_bounds__(256, SHORT || BK == 32 ? 4 : FM * FN == 64 ? 1 : 2)
 void product_kernel(ProductArgs p) {

@@ -19,4 +19,7 @@ def build_model(cfg: Config):
         cls = _REGISTRY[cfg.model]
     except KeyError:
         raise ValueError(f"unknown model {cfg.model!r}; have {sorted(_REGISTRY)}")
+    if cfg.fc_gate and cls is ResNet50:
+        raise ValueError("resnet50 has no hidden fully connected layers to "
+                         "gate; fc_gate must be empty")
     return cls(cfg)

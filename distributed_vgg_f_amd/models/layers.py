@@ -109,7 +109,11 @@ class MaxPool(nn.Module):
 
 
 class Dropout(nn.Module):
-    """Counter-based dropout: offset advances per call so steps decorrelate."""
+    """Counter-based dropout: offset advances per call so steps decorrelate.
+
+    The counter is the host's, so a captured graph would replay one mask; the
+    trainer runs such models eagerly. ops.dropout and ops.gated_linear also
+    take the offset from the device."""
 
     def __init__(self, p: float, seed: int = 0):
         super().__init__()

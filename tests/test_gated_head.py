@@ -48,6 +48,11 @@ def test_unknown_activation_is_refused():
         build_model(small(fc_gate="tanh"))
 
 
+def test_a_model_without_hidden_layers_refuses_a_gate():
+    with pytest.raises(ValueError, match="no hidden fully connected"):
+        build_model(small(model="resnet50", fc_gate="silu"))
+
+
 def test_layer_with_its_dropout():
     torch.manual_seed(0)
     layer, drop = GatedLinear(6, 8, "silu"), Dropout(0.5, seed=4)
