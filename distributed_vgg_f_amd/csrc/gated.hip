@@ -260,19 +260,25 @@ DEV s16x8 trade(f32x4 a, f32x4 b) {
 // tiles with the matrix cores busy for 70 % of the cycles. What bounds it
 // there is power: the more of them are busy, the lower the clock (1.75 GHz),
 // and 32x32x16 products took 917 and 970 us in place of 840 and 876. At 256 x
-// 9216 x 4096 the forward product (63 us, joined in 11) moves 151 MB of
-// weights and 34 of slabs; by count its tiles of 128 x 128 keep LDS busy for
-// two thirds of that time. A ring of four stages of 32 k, half as much again
-// in flight, came within 4 % either way over 26 shapes: latency is not the bound.
-template <class T, int MODE, int FM, int FN, int BK, bool SHORT = false>
-__global__ __launch_bounds__(256, SHORT || BK == 32 ? 4 : FM * FN == 64 ? 1 : 2)
+// 9216 x 4096 the forward product takes 59 us, joined in 8, for 151 MB of
+// weights and 17 of slabs (with weights that the last-level cache holds 43):
+// memory, at 2.9 TB/s, though wider reads of the weights (tiles of 64 x 256)
+// took 73.
+template <class T, int MODE, int FM, int FN, int BK, int RING,
+          bool SHORT = false>
+__global__ __launch_bounds__(256, SHORT || BK * RING == 64 ? 4
+                                  : RING == 4 || FM * FN == 64 ? 1 : 2)
 void product_kernel(ProductArgs p) {
   constexpr bool ATR = MODE == WGRAD, BTR = MODE != DGRAD;
   using TL = Tile<T, ATR, BTR, MODE == DGRAD ? 2 : 1, FM, FN, BK,
-                  MODE == FWD, SHORT>;
-  // two objects, so that reads of one do not wait for loads into the other
-  __shared__ __attribute__((aligned(1024))) char even[TL::STAGE];
-  __shared__ __attribute__((aligned(1024))) char odd[SHORT ? 16 : TL::STAGE];
+                  RING, MODE == FWD, SHORT>;
+  // an object each, so that reads of one do not wait for loads into others
+  constexpr int SECOND = SHORT ? 16 : TL::STAGE;
+  constexpr int MORE = RING == 4 ? TL::STAGE : 16;
+  __shared__ __attribute__((aligned(1024))) char lds0[TL::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds1[SECOND];
+  __shared__ __attribute__((aligned(1024))) char lds2[MORE];
+  __shared__ __attribute__((aligned(1024))) char lds3[MORE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -311,8 +317,8 @@ void product_kernel(ProductArgs p) {
     s.b[1][0] = p.b[1] + bn;
     s.b[1][1] = s.b[1][0] + bh;
   }
-  // parts of whole turns: two stages of 64 k, or one of each part
-  constexpr int TURN = MODE == DGRAD ? 64 : 128;
+  // parts of whole turns of the loop
+  constexpr int TURN = TL::TURN;
   const int turns = (p.k_len + TURN - 1) / TURN;
   const int each_ = turns / p.splits, more = turns % p.splits;
   s.k_first = (split * each_ + min(split, more)) * TURN;
@@ -320,7 +326,12 @@ void product_kernel(ProductArgs p) {
 
   f32x4 acc[FM][FN];
   TL tile;
-  tile.run((lds_char*)even, (lds_char*)odd, s, wave, lane, acc);
+  Bufs buf;
+  buf.b0 = (lds_char*)lds0;
+  buf.b1 = (lds_char*)lds1;
+  buf.b2 = (lds_char*)lds2;
+  buf.b3 = (lds_char*)lds3;
+  tile.run(buf, s, wave, lane, acc);
 
   // Straight from the accumulators: a trip through LDS for wider stores took
   // 5 us a 256 x 256 tile, of 14 in all besides its products. Lane (c, q):
@@ -381,9 +392,9 @@ void product_kernel(ProductArgs p) {
       // 16.5 us, through LDS in pieces of 32 rows 14.2, and in this form, 64
       // rows of a wave at a time, which is all of the LDS, in a loop that has
       // the next read under way, 12.8. 16-byte chunks trade places by row.
-      static_assert(TL::STAGE == 65536, "32 KB a wave");
+      static_assert(TL::STAGE == 65536 && RING == 2, "32 KB a wave");
       __syncthreads();
-      float* mine = reinterpret_cast<float*>((wave & 2 ? odd : even) +
+      float* mine = reinterpret_cast<float*>((wave & 2 ? lds1 : lds0) +
                                              (wave & 1) * 32768);
       const u32 off = o.drop ? o.d.off() : 0;
       const int n = nw + (lane & 7) * 8;
@@ -892,26 +903,35 @@ static i64 ld_of(const at::Tensor& t) {
 
 constexpr int ROWS_MAX = 16, ROWS_TARGET = 256;
 
-struct Plan { int fm, fn, bk, splits, tiles_m, tiles_n; bool brief; };
+struct Plan { int fm, fn, bk, ring, splits, tiles_m, tiles_n; bool brief; };
 
 // Which tile, and into how many parts the contraction is split: the least
 // time by a model of what the tiles measured over the 138 products of 46
-// shapes of 17 to 8192 rows and 64 to 25088 columns (it is off by 16 % there;
-// what it picks is 2 % slower than the best of all tiles and splits in the
-// mean, 20 % at worst).
+// shapes of 17 to 8192 rows and 64 to 25088 columns (it is off by 13 % there;
+// what it picks is 1.5 % slower than the best of all tiles and splits in the
+// mean, 10 % at worst).
 // Microseconds. A stage costs `one` if a tile has its CU to itself and `all`
 // if the CU is full; `edge` is a tile's first loads and its epilogue.
+// Four buffers are for launches of about one tile a CU: two leave such a tile
+// waiting for memory at every stage (0.69 and 0.61 us in place of 0.52 and
+// 0.38; 2048 x 4096 x 1000: 51.4 -> 39.2, 512 x 4096 x 4096: 54.3 -> 46.3).
+// Two tiles on a CU cover for each other, and then two buffers each are the
+// faster (797 x 5368 x 3032: 91 us, with four buffers 107).
 static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
-  struct Kind { int fm, fn, bk, per_cu; double one, all, edge; bool brief; };
-  static const Kind kinds[] = {{8, 8, 64, 1, 1.24, 1.24, 9.8, false},
-                               {4, 4, 64, 2, 0.69, 0.96, 3.9, false},
-                               {2, 4, 64, 3, 0.61, 0.93, 2.8, false},
-                               {4, 4, 32, 4, 0.69, 1.85, 4.0, false},
-                               {4, 4, 64, 4, 0.69, 1.85, 3.9, true}};
+  struct Kind {
+    int fm, fn, bk, ring, per_cu;
+    double one, all, edge;
+    bool brief;
+  };
+  static const Kind kinds[] = {{8, 8, 64, 2, 1, 1.24, 1.24, 9.8, false},
+                               {4, 4, 64, 2, 2, 0.69, 0.96, 3.9, false},
+                               {4, 4, 64, 4, 1, 0.52, 0.52, 3.7, false},
+                               {2, 4, 64, 2, 3, 0.61, 0.93, 2.8, false},
+                               {2, 4, 64, 4, 1, 0.38, 0.38, 2.8, false},
+                               {4, 4, 32, 2, 4, 0.69, 1.85, 4.0, false},
+                               {4, 4, 64, 2, 4, 0.69, 1.85, 3.9, true}};
   constexpr double CUS = 256, MEM = 4.5e6, JOIN_MEM = 7e6;
   const double join = mode == FWD ? 4.0 : 2.4;
-  // turns of the loop, and stages in each
-  const int turns = ceil_div(k_len, mode == DGRAD ? 64 : 128);
   const double mats = mode == DGRAD ? 1 : 2;
   const double out = double(rows) * cols;
   // bytes that the product moves at least
@@ -929,6 +949,9 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
     const int tm = ceil_div(rows, 32 * k.fm);
     const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
                    (mode == WGRAD ? 2 : 1);
+    // turns of the loop: a stage in each buffer (of 64 k: stages of 32 k come
+    // two at a time), of DGRAD's two parts in turns
+    const int turns = ceil_div(k_len, 64 * k.ring / (mode == DGRAD ? 2 : 1));
     // 1 2 3 4 6 8 12 16 24 32
     for (int sp = 1; sp <= turns && sp <= 32;
          sp += sp < 4 ? 1 : sp & (sp - 1) ? sp / 3 : sp / 2) {
@@ -936,7 +959,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
       // a launch holds less than 2^32 threads; tiles of 256 x 128 and wider,
       // unsplit, stay below this for whatever fits in memory
       if (wgs > (1 << 23) && !(k.fm == 8 && sp == 1)) continue;
-      const double depth = k.brief ? 1 : 2 * ceil_div(turns, sp);
+      const double depth = k.brief ? 1 : k.ring * ceil_div(turns, sp);
       auto round = [&](double n) {
         const double share = k.per_cu > 1
             ? (std::ceil(n / CUS) - 1) / (k.per_cu - 1) : 1;
@@ -948,7 +971,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
       if (sp > 1) t += join + sp * mats * out * 8 / JOIN_MEM;
       if (least == 0 || t < least) {
         least = t;
-        best = Plan{k.fm, k.fn, k.bk, sp, tm, tn, k.brief};
+        best = Plan{k.fm, k.fn, k.bk, k.ring, sp, tm, tn, k.brief};
       }
     }
   }
@@ -960,22 +983,24 @@ static void launch(const Plan& pl, const ProductArgs& a) {
   dim3 grid(u32(pl.tiles_m) * pl.tiles_n * pl.splits);
   auto st = cur_stream();
   if (pl.brief) {
-    hipLaunchKernelGGL((product_kernel<T, WGRAD, 4, 4, 64, true>), grid,
+    hipLaunchKernelGGL((product_kernel<T, WGRAD, 4, 4, 64, 2, true>), grid,
                        dim3(256), 0, st, a);
     HIP_CHECK(hipGetLastError());
     return;
   }
-#define TILE_CASE(FM, FN, BK)                                              \
-  if (pl.fm == FM && pl.fn == FN && pl.bk == BK) {                         \
-    hipLaunchKernelGGL((product_kernel<T, MODE, FM, FN, BK>), grid,        \
+#define TILE_CASE(FM, FN, BK, RING)                                        \
+  if (pl.fm == FM && pl.fn == FN && pl.bk == BK && pl.ring == RING) {      \
+    hipLaunchKernelGGL((product_kernel<T, MODE, FM, FN, BK, RING>), grid,  \
                        dim3(256), 0, st, a);                               \
     HIP_CHECK(hipGetLastError());                                          \
     return;                                                                \
   }
-  TILE_CASE(8, 8, 64)
-  TILE_CASE(4, 4, 64)
-  TILE_CASE(2, 4, 64)
-  if constexpr (MODE == WGRAD) { TILE_CASE(4, 4, 32) }
+  TILE_CASE(8, 8, 64, 2)
+  TILE_CASE(4, 4, 64, 2)
+  TILE_CASE(4, 4, 64, 4)
+  TILE_CASE(2, 4, 64, 2)
+  TILE_CASE(2, 4, 64, 4)
+  if constexpr (MODE == WGRAD) { TILE_CASE(4, 4, 32, 2) }
 #undef TILE_CASE
   TORCH_CHECK(false, "gated_linear: no tile of this size");
 }

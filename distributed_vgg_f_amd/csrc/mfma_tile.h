@@ -10,10 +10,10 @@
 // 32 k a wave reads 16 (FM + FN) rows of 64 bytes for FM FN products of 16
 // cycles, 64 B/cycle of the CU's 128 at 8 x 8, but 96 for 8 waves of 8 x 4.
 //
-// Stages of 64 (or 32) k go straight from memory to LDS (16 bytes a lane), two deep;
-// the fragments of the next 32 k are read while the present ones multiply, so
-// a stage costs one barrier. Buffer loads put zeros where rows, columns or
-// the contraction end.
+// Stages of 64 (or 32) k go straight from memory to LDS (16 bytes a lane), into
+// two buffers in turn or four; the fragments of the next 32 k are read while
+// the present ones multiply, so a stage costs one barrier. Buffer loads put
+// zeros where rows, columns or the contraction end.
 #pragma once
 
 #include "common.h"
@@ -159,6 +159,16 @@ struct Frags {
   }
 };
 
+// The stages' buffers: up to four objects, so that reads of one do not wait for
+// loads into the others. (An array of them would become a constant in memory.)
+struct Bufs {
+  lds_char *b0, *b1, *b2, *b3;
+  template <int N>
+  DEV lds_char* at() const {
+    return N == 0 ? b0 : N == 1 ? b1 : N == 2 ? b2 : b3;
+  }
+};
+
 constexpr int max_(int a, int b) { return a > b ? a : b; }
 
 // What one tile multiplies. The contraction may come in two parts with
@@ -172,6 +182,8 @@ struct TileSrc {
   int k_first, k_last;      // the contraction [k_first, k_last) of each part
 };
 
+// RING: buffers, 2 or 4. With four, three stages are under way while one is
+// multiplied, and a tile needs no other on its CU to cover for it.
 // BK: k of a stage. Stages of 64 take a barrier for every two steps of 32
 // and keep rows of 128 bytes together; stages of 32 take half the LDS, and
 // more tiles share a CU.
@@ -179,7 +191,7 @@ struct TileSrc {
 // one. SHORT: the whole contraction is one stage, which then is all the LDS
 // that the tile needs; more tiles share a CU.
 template <class T, bool ATR, bool BTR, int PARTS, int FM, int FN, int BK,
-          bool PAIRED, bool SHORT>
+          int RING, bool PAIRED, bool SHORT>
 struct Tile {
   static constexpr int BM = 32 * FM, BN = 32 * FN, HALF = BN / 2;
   using PA = Panel<ATR, BM, BK>;
@@ -268,15 +280,17 @@ struct Tile {
           }
         }
       }
-      if (FILL && i == ROW0 - 1) sync();
+      if (FILL && i == ROW0 - 1) sync<(RING - 2) * LOADS>();
     }
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // this wave's loads have landed and its reads are done; then all waves'
+  // this wave's loads have landed but for the last LEFT, and its reads are
+  // done; then all waves'
+  template <int LEFT>
   DEV static void sync() {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(LEFT) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -285,12 +299,9 @@ struct Tile {
   // acc[i][j]: rows 16 i + lane % 16 of the wave's 16 FM; columns
   // 16 (j % FH) + 4 (lane / 16) + 0..3 of the wave's in half j / FH (PAIRED)
   // or in its own half.
-  DEV void run(lds_char* even, lds_char* odd, const TileSrc& s, int wave_,
+  DEV void run(const Bufs& buf, const TileSrc& s, int wave_,
                int lane, f32x4 (&acc)[FM][FN]) {
-    constexpr int P1 = PARTS - 1;
     constexpr int LASTH = BK / 32 - 1;          // last half of a stage
-    constexpr int KODD = PARTS == 2 ? 0 : BK;   // k of the odd stage
-    constexpr int KTURN = KODD + BK;            // k of a turn of two
     wave = wave_;
     pa.init(wave, lane, s.lda, s.rows_a);
     pb[0].init(wave, lane, s.ldb, s.rows_b[0]);
@@ -304,34 +315,46 @@ struct Tile {
         acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         asm volatile("" : "+a"(acc[i][j]));   // here, not just before its use
       }
+    first<0>(buf, s);
+    sync<(SHORT ? 0 : RING - 1) * LOADS>();
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) load<0>(s, even, s.k_first, l);
-    if (!SHORT) {
+    for (int j = 0; j < FN; ++j) fetch_b(buf.template at<0>(), 0, 0, j);
 #pragma unroll
-      for (int l = 0; l < LOADS; ++l) load<P1>(s, odd, s.k_first + KODD, l);
-    }
-    sync();
-#pragma unroll
-    for (int j = 0; j < FN; ++j) fetch_b(even, 0, 0, j);
-#pragma unroll
-    for (int i = 0; i < FM - 1; ++i) fetch_a(even, 0, i);
-    if (SHORT) {
-      if (BK == 64) step<PLAIN, 0, 0>(s, even, 0, even, 1, even, 0, acc);
-      step<LAST, LASTH, 0>(s, even, LASTH, even, 0, even, 0, acc);
+    for (int i = 0; i < FM - 1; ++i) fetch_a(buf.template at<0>(), 0, i);
+    if constexpr (SHORT) {
+      if (BK == 64) step<PLAIN, 0, 0>(s, buf.template at<0>(), 0, buf.template at<0>(), 1, buf.template at<0>(), 0, acc);
+      step<LAST, LASTH, 0>(s, buf.template at<0>(), LASTH, buf.template at<0>(), 0, buf.template at<0>(), 0, acc);
     } else {
-      // turns of two stages: an odd last one is followed by zeros
-      for (int k = s.k_first; k < s.k_last; k += KTURN) {
-        if (BK == 64) step<PLAIN, 0, 0>(s, even, 0, even, 1, even, 0, acc);
-        step<REFILL, LASTH, 0>(s, even, LASTH, odd, 0, even, k + KTURN, acc);
-        if (BK == 64) step<PLAIN, 0, 0>(s, odd, 0, odd, 1, odd, 0, acc);
-        step<REFILL, 1, P1>(s, odd, LASTH, even, 0, odd, k + KTURN + KODD,
-                            acc);
+      // turns of all buffers: missing last stages are zeros
+      for (int k = s.k_first; k < s.k_last; k += TURN) {
+        stages<0>(buf, s, k, acc);
         mfma_wait();        // behind the loop accumulators may be moved
       }
     }
     // zeros still on their way must not land in what comes after
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     mfma_done(acc);
+  }
+
+  // k of a turn of all buffers, and where in it buffer n is
+  static constexpr int TURN = RING * BK / PARTS;
+  static constexpr int k_of(int n) { return n / PARTS * BK; }
+  template <int N>
+  DEV void first(const Bufs& buf, const TileSrc& s) {
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l)
+      load<N % PARTS>(s, buf.template at<N>(), s.k_first + k_of(N), l);
+    if constexpr (!SHORT && N + 1 < RING) first<N + 1>(buf, s);
+  }
+  template <int N>
+  DEV void stages(const Bufs& buf, const TileSrc& s, int k,
+                  f32x4 (&acc)[FM][FN]) {
+    constexpr int LASTH = BK / 32 - 1, NEXT = (N + 1) % RING;
+    if constexpr (BK == 64)
+      step<PLAIN, 0, N % PARTS>(s, buf.template at<N>(), 0, buf.template at<N>(), 1, buf.template at<N>(), 0, acc);
+    step<REFILL, BK == 64 ? 1 : N & 1, N % PARTS>(
+        s, buf.template at<N>(), LASTH, buf.template at<NEXT>(), 0, buf.template at<N>(), k + TURN + k_of(N), acc);
+    if constexpr (N + 1 < RING) stages<N + 1>(buf, s, k, acc);
   }
 };
 
