@@ -250,6 +250,26 @@ def test_more_tiles_than_the_card_holds(M, K, N):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N,act", [
+    (1999, 520, 2056, "silu"),
+    (2003, 1001, 4100, "gelu"),
+    (2056, 4104, 1003, "gelu_tanh"),
+    (4101, 1000, 2056, "sigmoid"),
+    (2003, 4104, 520, "relu"),
+    (4101, 136, 4104, "silu"),
+    (4100, 2056, 1031, "gelu"),
+    (2051, 4104, 136, "gelu_tanh"),
+    (1030, 2056, 2056, "sigmoid"),
+    (4099, 4104, 40, "relu"),
+    (520, 1000, 1032, "silu"), (60, 2056, 4104, "gelu")])
+def test_every_tile_whole_and_split(M, K, N, act, dtype):
+    """Sizes that between them take each tile of each product, with the
+    contraction in one part and in several."""
+    check_case(M, K, N, dtype, act, True, 0.5)
+
+
+@gpu
 def test_fused_dropout_is_the_dropout_of_the_result():
     for n in (200, 199):
         ts = [None if t is None else t.to(DEV)
