@@ -45,7 +45,8 @@ def gated_linear(x, w_gate, w_up, bias_gate=None, bias_up=None,
 
     GPU: bf16 or fp16, one type and one device for all operands, any K, N
     and strides; sums in 32 bits. Operands whose rows do not start on 16
-    bytes are copied to rows that do, once a call. Differentiates once.
+    bytes are copied to rows that do, once a call (not for answers of up to
+    16 rows). Differentiates once.
     """
     if act not in _ACT_ID:
         raise ValueError(f"gated_linear: unknown activation {act!r}; have "

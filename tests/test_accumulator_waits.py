@@ -68,7 +68,7 @@ def too_early(code):
     return bad
 
 
-def test_checker_sees_planted_mistakes():
+def test_the_scan_sees_planted_mistakes():
     mfma = "v_mfma_f32_16x16x32_bf16 a[0:3], v[0:3], v[4:7], a[0:3]"
     read = "v_accvgpr_read_b32 v9, a2"
     far = [(8 * i, t, None) for i, t in enumerate([mfma, "s_nop 10", read])]

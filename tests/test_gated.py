@@ -251,6 +251,30 @@ def test_more_tiles_than_the_card_holds(M, K, N):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [(1, 1, 8), (1, 33, 9), (16, 31, 127),
+                                   (3, 300, 129), (5, 1055, 135),
+                                   (16, 64, 137), (2, 4097, 259),
+                                   (1, 520, 4095), (7, 2049, 1000)])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_answers_from_rows_that_start_anywhere(M, K, N, dtype, p):
+    # each operand a part of a matrix that is NaN around it
+    ts = make(M, K, N, dtype, True)
+    factor = keep_mask((M, N), p, 7, 3).double() / (1 - p) if p else 1.0
+    outs, errs = oracle(*ts, "gelu", factor)
+    parts = []
+    for t in ts[:3]:
+        big = torch.full((t.shape[0] + 2, t.shape[1] + 13), float("nan"),
+                         dtype=dtype, device=DEV)
+        part = big[1:-1, 3:-10]
+        part.copy_(t)
+        parts.append(part)
+    h = ops.gated_linear(*parts, ts[3].to(DEV), ts[4].to(DEV), act="gelu",
+                         p=p, seed=7, offset=3)
+    compare([h], outs, errs, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,K,N,act", [
     (1999, 520, 2056, "silu"),
     (2003, 1001, 4100, "gelu"),
