@@ -994,10 +994,12 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
   Plan best{};
   double least = 0;
   for (const Kind& k : kinds) {
-    // Stages of 32 k pay only where both operands lie along their rows, and
-    // contractions are short (256 x 9216 x 4096: 73.5 -> 60.3 us); else their
-    // rows of 64 bytes cost more than four tiles a CU gain.
-    if (k.bk == 32 && mode != WGRAD) continue;
+    // Stages of 32 k pay where both operands lie along their rows and
+    // contractions are short (256 x 9216 x 4096: 73.5 -> 60.3 us), and for dX
+    // of up to 96 columns of G, which leave half of a wider turn empty (8072 x
+    // 12800 x 96: 84.5 -> 67.7; at 128 columns 18.4 and 18.7); else their rows
+    // of 64 bytes cost more than four tiles a CU gain.
+    if (k.bk == 32 && mode != WGRAD && (mode != DGRAD || k_len > 96)) continue;
     if (k.brief && (mode != WGRAD || k_len > 64)) continue;
     const int tm = ceil_div(rows, 32 * k.fm);
     const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
@@ -1053,7 +1055,7 @@ static void launch(const Plan& pl, const ProductArgs& a) {
   TILE_CASE(4, 4, 64, 4)
   TILE_CASE(2, 4, 64, 2)
   TILE_CASE(2, 4, 64, 4)
-  if constexpr (MODE == WGRAD) { TILE_CASE(4, 4, 32, 2) }
+  if constexpr (MODE != FWD) { TILE_CASE(4, 4, 32, 2) }
 #undef TILE_CASE
   TORCH_CHECK(false, "gated_linear: no tile of this size");
 }

@@ -286,7 +286,8 @@ def test_answers_from_rows_that_start_anywhere(M, K, N, dtype, p):
     (2051, 4104, 136, "gelu_tanh"),
     (1030, 2056, 2056, "sigmoid"),
     (4099, 4104, 40, "relu"),
-    (520, 1000, 1032, "silu"), (60, 2056, 4104, "gelu")])
+    (520, 1000, 1032, "silu"), (60, 2056, 4104, "gelu"),
+    (1030, 8200, 90, "silu")])
 def test_every_tile_whole_and_split(M, K, N, act, dtype):
     """Sizes that between them take each tile of each product, with the
     contraction in one part and in several."""
