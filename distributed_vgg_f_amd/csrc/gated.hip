@@ -64,8 +64,8 @@ DEV f32x8 act8(int act, f32x8 g, f32x8& d) {
       d = each(g, [](float v, int) { return v <= 0.f ? 0.f : 1.f; });
       return each(g, [](float v, int) { return v <= 0.f ? 0.f : v; });
     case GELU:
-      // erfc(x) = t (a1 + t (a2 + ... a5)) exp(-x^2), t = 1 / (1 + p x), x >= 0,
-      // off by at most 1.5e-7 (Abramowitz and Stegun, 7.1.26); its
+      // erfc(x) = t (a1 + t (a2 + ... a5)) exp(-x^2), t = 1 / (1 + p x), for
+      // x >= 0, off by at most 1.5e-7 (Abramowitz and Stegun, 7.1.26); its
       // exponential serves the derivative too. erfcf took 10 us more a round
       // of 256 tiles of 256 x 128.
       return each(g, [&](float v, int r) {
@@ -1179,8 +1179,9 @@ static DropArgs gated_drop(const at::Tensor& x, double p, int64_t seed,
 __global__ void copy_offset_kernel(const i64* in, i64* out) { *out = *in; }
 
 // Returns h [M][N], and with `train` also what backward wants: G and U as
-// one [2][M][N up to a vector] in 32 bits, the three operands as the tiles load them,
-// and the offset that the mask was drawn with if it came from the device.
+// one [2][M][N up to a vector] in 32 bits, the three operands as the tiles
+// load them, and the offset that the mask was drawn with if it came from the
+// device.
 std::vector<at::Tensor> gated_fwd(
     const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
     const c10::optional<at::Tensor>& bg, const c10::optional<at::Tensor>& bu,

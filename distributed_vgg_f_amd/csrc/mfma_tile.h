@@ -318,12 +318,13 @@ struct Tile {
     first<0>(buf, s);
     sync<(SHORT ? 0 : RING - 1) * LOADS>();
 #pragma unroll
-    for (int j = 0; j < FN; ++j) fetch_b(buf.template at<0>(), 0, 0, j);
+    for (int j = 0; j < FN; ++j) fetch_b(buf.at<0>(), 0, 0, j);
 #pragma unroll
-    for (int i = 0; i < FM - 1; ++i) fetch_a(buf.template at<0>(), 0, i);
+    for (int i = 0; i < FM - 1; ++i) fetch_a(buf.at<0>(), 0, i);
     if constexpr (SHORT) {
-      if (BK == 64) step<PLAIN, 0, 0>(s, buf.template at<0>(), 0, buf.template at<0>(), 1, buf.template at<0>(), 0, acc);
-      step<LAST, LASTH, 0>(s, buf.template at<0>(), LASTH, buf.template at<0>(), 0, buf.template at<0>(), 0, acc);
+      lds_char* one = buf.at<0>();
+      if (BK == 64) step<PLAIN, 0, 0>(s, one, 0, one, 1, one, 0, acc);
+      step<LAST, LASTH, 0>(s, one, LASTH, one, 0, one, 0, acc);
     } else {
       // turns of all buffers: missing last stages are zeros
       for (int k = s.k_first; k < s.k_last; k += TURN) {
@@ -343,17 +344,18 @@ struct Tile {
   DEV void first(const Bufs& buf, const TileSrc& s) {
 #pragma unroll
     for (int l = 0; l < LOADS; ++l)
-      load<N % PARTS>(s, buf.template at<N>(), s.k_first + k_of(N), l);
+      load<N % PARTS>(s, buf.at<N>(), s.k_first + k_of(N), l);
     if constexpr (!SHORT && N + 1 < RING) first<N + 1>(buf, s);
   }
   template <int N>
   DEV void stages(const Bufs& buf, const TileSrc& s, int k,
                   f32x4 (&acc)[FM][FN]) {
     constexpr int LASTH = BK / 32 - 1, NEXT = (N + 1) % RING;
+    lds_char* now = buf.at<N>();
     if constexpr (BK == 64)
-      step<PLAIN, 0, N % PARTS>(s, buf.template at<N>(), 0, buf.template at<N>(), 1, buf.template at<N>(), 0, acc);
+      step<PLAIN, 0, N % PARTS>(s, now, 0, now, 1, now, 0, acc);
     step<REFILL, BK == 64 ? 1 : N & 1, N % PARTS>(
-        s, buf.template at<N>(), LASTH, buf.template at<NEXT>(), 0, buf.template at<N>(), k + TURN + k_of(N), acc);
+        s, now, LASTH, buf.at<NEXT>(), 0, now, k + TURN + k_of(N), acc);
     if constexpr (N + 1 < RING) stages<N + 1>(buf, s, k, acc);
   }
 };

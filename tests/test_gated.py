@@ -3,8 +3,9 @@
 Bounds. With e = half a step of the operands' type and E = 2^-24, K products
 summed in 32 bits are off by at most (K + 4) E times the sum of their
 magnitudes (K additions, the product, the bias). Backward works on G and U in
-32 bits, rounds dG and dU once (e) and its results once (e); each error is carried through the formulas by the largest slope of
-the function that it passes. The 32-bit activations are off by at most 2^-19
+32 bits, rounds dG and dU once (e) and its results once (e); each error is
+carried through the formulas by the largest slope of the function that it
+passes. The 32-bit activations are off by at most 2^-19
 of max(1, |g|): their exponential multiplies its argument's error of E |g|.
 """
 
