@@ -15,7 +15,7 @@
 // bits, and so do G and U kept for the backward pass: rounded to 16 they
 // nearly double the error of the gradients (bf16, 256 x 9216 x 4096: 0.0031
 // of their size instead of 0.0024, one rounding of the result being 0.0017),
-// and they are 4 % of the time at the largest sizes, less elsewhere. dG and
+// and they are 3 to 4 % of the time at the largest sizes, less elsewhere. dG and
 // dU are rounded to the type of x, which the matrix instructions take.
 
 #include <torch/extension.h>
