@@ -1,8 +1,10 @@
-// Autograd nodes of the operators in dropout.hip and gated.hip. In C++ because
-// the small calls are bound by what the host does: 256 x 4096 dropout forward
-// and backward took 31 us with nodes in Python for two kernels of 3 us.
+// Autograd nodes of the operators in dropout.hip and gated.hip, and their
+// entries in the dispatcher. In C++ because the small calls are bound by what
+// the host does: 256 x 4096 dropout forward and backward took 31 us with nodes
+// in Python for two kernels of 3 us.
 
 #include <torch/extension.h>
+#include <torch/library.h>
 
 namespace dvgg {
 
@@ -23,6 +25,13 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 using OptTensor = c10::optional<at::Tensor>;
+
+// Wrappers of function transforms (vmap, torch.func) have no memory of their
+// own for a kernel to read.
+static void check_memory(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.has_storage(), name, ": takes tensors with memory of their "
+              "own, no function transforms (vmap, torch.func)");
+}
 
 // Backward draws the mask again from (p, seed, offset) and runs the forward's
 // kernel on dy. An offset from the device comes back from the kernel as the
@@ -59,6 +68,20 @@ at::Tensor dropout_ad(const at::Tensor& x, double p, int64_t seed,
   if (at::GradMode::is_enabled() && x.requires_grad())
     return DropoutFn::apply(x, p, seed, offset, offset_t);
   return dropout(x.contiguous(), p, seed, offset, offset_t)[0];
+}
+
+// The dispatcher's entries: what records calls (torch.jit.trace) sees one
+// operator, dvgg::dropout or dvgg::gated_linear, and replays it. Called past
+// the dispatcher, the kernel would leave no trace but the empty buffer that it
+// fills.
+at::Tensor dropout_call(const at::Tensor& x, double p, int64_t seed,
+                        int64_t offset, const OptTensor& offset_t) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("dvgg::dropout", "")
+          .typed<at::Tensor(const at::Tensor&, double, int64_t, int64_t,
+                            const OptTensor&)>();
+  check_memory(x, "dropout");
+  return op.call(x, p, seed, offset, offset_t);
 }
 
 // Keeps both projections; backward is one pass over them and two products.
@@ -127,14 +150,48 @@ at::Tensor gated_ad(const at::Tensor& x, const at::Tensor& wg,
                     const at::Tensor& wu, const OptTensor& bg,
                     const OptTensor& bu, int64_t act, double p, int64_t seed,
                     int64_t offset, const OptTensor& offset_t,
-                    const std::vector<OptTensor>& outs) {
+                    const OptTensor& wg_grad, const OptTensor& wu_grad,
+                    const OptTensor& bg_grad, const OptTensor& bu_grad) {
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || wg.requires_grad() || wu.requires_grad() ||
        (bg && bg->requires_grad()) || (bu && bu->requires_grad())))
-    return GatedFn::apply(x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
-                          outs);
+    return GatedFn::apply(
+        x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
+        std::vector<OptTensor>{wg_grad, wu_grad, bg_grad, bu_grad});
   return gated_fwd(x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
                    false)[0];
+}
+
+at::Tensor gated_call(const at::Tensor& x, const at::Tensor& wg,
+                      const at::Tensor& wu, const OptTensor& bg,
+                      const OptTensor& bu, int64_t act, double p,
+                      int64_t seed, int64_t offset, const OptTensor& offset_t,
+                      const std::vector<OptTensor>& outs) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("dvgg::gated_linear", "")
+          .typed<at::Tensor(const at::Tensor&, const at::Tensor&,
+                            const at::Tensor&, const OptTensor&,
+                            const OptTensor&, int64_t, double, int64_t,
+                            int64_t, const OptTensor&, const OptTensor&,
+                            const OptTensor&, const OptTensor&,
+                            const OptTensor&)>();
+  TORCH_CHECK(outs.size() == 4, "gated_linear: four gradient buffers or None");
+  for (auto* t : {&x, &wg, &wu}) check_memory(*t, "gated_linear");
+  for (auto* t : {&bg, &bu}) if (*t) check_memory(**t, "gated_linear");
+  return op.call(x, wg, wu, bg, bu, act, p, seed, offset, offset_t, outs[0],
+                 outs[1], outs[2], outs[3]);
+}
+
+// without a key: one kernel for every pass through the dispatcher, which
+// makes its autograd node itself
+TORCH_LIBRARY(dvgg, m) {
+  m.def("dropout(Tensor x, float p, int seed, int offset, "
+        "Tensor? offset_t=None) -> Tensor", dropout_ad);
+  m.def("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, "
+        "Tensor? bias_gate, Tensor? bias_up, int act, float p, int seed, "
+        "int offset, Tensor? offset_t=None, Tensor? w_gate_grad=None, "
+        "Tensor? w_up_grad=None, Tensor? bias_gate_grad=None, "
+        "Tensor? bias_up_grad=None) -> Tensor", gated_ad);
 }
 
 }  // namespace dvgg

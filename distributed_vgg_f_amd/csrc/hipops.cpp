@@ -36,13 +36,13 @@ std::vector<at::Tensor> dropout_fwd(const at::Tensor&, double, int64_t,
 at::Tensor dropout_bwd(const at::Tensor&, const at::Tensor&, double);
 
 // fn.cpp
-at::Tensor dropout_ad(const at::Tensor&, double, int64_t, int64_t,
-                      const c10::optional<at::Tensor>&);
-at::Tensor gated_ad(const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                    const c10::optional<at::Tensor>&,
-                    const c10::optional<at::Tensor>&, int64_t, double,
-                    int64_t, int64_t, const c10::optional<at::Tensor>&,
-                    const std::vector<c10::optional<at::Tensor>>&);
+at::Tensor dropout_call(const at::Tensor&, double, int64_t, int64_t,
+                        const c10::optional<at::Tensor>&);
+at::Tensor gated_call(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                      const c10::optional<at::Tensor>&,
+                      const c10::optional<at::Tensor>&, int64_t, double,
+                      int64_t, int64_t, const c10::optional<at::Tensor>&,
+                      const std::vector<c10::optional<at::Tensor>>&);
 
 // lrnpool.hip
 at::Tensor lrn_fwd(const at::Tensor&, int64_t, double, double, double);
@@ -95,10 +95,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bump_weight_gen", &dvgg::bump_weight_gen);
   m.def("dropout_fwd", &dvgg::dropout_fwd);
   m.def("dropout_bwd", &dvgg::dropout_bwd);
-  m.def("dropout", &dvgg::dropout_ad, py::arg("x"), py::arg("p"),
+  m.def("dropout", &dvgg::dropout_call, py::arg("x"), py::arg("p"),
         py::arg("seed"), py::arg("offset"),
         py::arg("offset_t") = c10::nullopt);
-  m.def("gated_linear", &dvgg::gated_ad, py::arg("x"), py::arg("w_gate"),
+  m.def("gated_linear", &dvgg::gated_call, py::arg("x"), py::arg("w_gate"),
         py::arg("w_up"), py::arg("bias_gate"), py::arg("bias_up"),
         py::arg("act"), py::arg("p"), py::arg("seed"), py::arg("offset"),
         py::arg("offset_t"), py::arg("grad_outs"));
