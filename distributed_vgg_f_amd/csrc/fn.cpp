@@ -33,6 +33,12 @@ static void check_memory(const at::Tensor& t, const char* name) {
               "own, no function transforms (vmap, torch.func)");
 }
 
+// A tangent would be lost without a word: the kernels do not see it.
+static void check_tangent(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, ": no "
+                              "forward-mode differentiation, only backward");
+}
+
 // Backward draws the mask again from (p, seed, offset) and runs the forward's
 // kernel on dy. An offset from the device comes back from the kernel as the
 // value that it drew with: the caller may count the tensor up meanwhile.
@@ -55,16 +61,19 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
     const int64_t seed = ctx->saved_data["seed"].toInt();
     const int64_t offset = ctx->saved_data["offset"].toInt();
     Variable dx;
-    if (grads[0].defined())
+    if (grads[0].defined()) {
+      check_tangent(grads[0], "dropout");
       dx = at::GradMode::is_enabled()
                ? DropoutFn::apply(grads[0], p, seed, offset, used)
                : dropout(grads[0].contiguous(), p, seed, offset, used)[0];
+    }
     return {dx, Variable(), Variable(), Variable(), Variable()};
   }
 };
 
 at::Tensor dropout_ad(const at::Tensor& x, double p, int64_t seed,
                       int64_t offset, const OptTensor& offset_t) {
+  check_tangent(x, "dropout");
   if (at::GradMode::is_enabled() && x.requires_grad())
     return DropoutFn::apply(x, p, seed, offset, offset_t);
   return dropout(x.contiguous(), p, seed, offset, offset_t)[0];
@@ -126,6 +135,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
         need |= int64_t(1) << i;
     variable_list result(11);
     if (!grads[0].defined()) return result;
+    check_tangent(grads[0], "gated_linear");
     std::vector<OptTensor> outs(5);
     for (int i = 0; i < 4; ++i) {
       auto it = d.find(OUT[i]);
@@ -152,6 +162,8 @@ at::Tensor gated_ad(const at::Tensor& x, const at::Tensor& wg,
                     int64_t offset, const OptTensor& offset_t,
                     const OptTensor& wg_grad, const OptTensor& wu_grad,
                     const OptTensor& bg_grad, const OptTensor& bu_grad) {
+  for (auto* t : {&x, &wg, &wu}) check_tangent(*t, "gated_linear");
+  for (auto* t : {&bg, &bu}) if (*t) check_tangent(**t, "gated_linear");
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || wg.requires_grad() || wu.requires_grad() ||
        (bg && bg->requires_grad()) || (bu && bu->requires_grad())))

@@ -3,6 +3,7 @@ recording a call and replaying it, function transforms."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from distributed_vgg_f_amd import ops
 from distributed_vgg_f_amd.models.layers import Dropout, hidden_fc, run_hidden
@@ -98,3 +99,49 @@ def test_function_transforms_are_refused():
         torch.func.vmap(lambda w: ops.gated_linear(x, w, wu))(wg[None])
     with pytest.raises(RuntimeError, match="no function transforms"):
         torch.func.grad(lambda t: ops.dropout(t, 0.5, 1, 1).sum())(x.float())
+
+
+def dual_calls(dev):
+    """Calls with one operand that carries a tangent, none with a gradient."""
+    ext = ops.native.ext()
+    x, w = torch.ones(4, 8, device=dev), torch.ones(8, 8, device=dev)
+    half, b = [t.bfloat16() for t in (x, w)], torch.ones(8, device=dev)
+
+    def gated(which):
+        ts = [half[0], half[1], half[1].clone(), b.bfloat16(), b.bfloat16()]
+        ts[which] = fwAD.make_dual(ts[which], torch.ones_like(ts[which]))
+        return ext.gated_linear(*ts, 0, 0.0, 0, 0, None, [None] * 4)
+    return [lambda: ext.dropout(fwAD.make_dual(x, x), 0.5, 1, 1)] + \
+        [lambda i=i: gated(i) for i in range(5)]
+
+
+@pytest.mark.skipif(not ops.native.available(),
+                    reason="needs the built extension")
+@pytest.mark.parametrize("which", range(6))
+def test_tangents_are_refused(which):
+    # before anything asks for a GPU, so here too
+    with fwAD.dual_level(), pytest.raises(NotImplementedError,
+                                          match="no forward-mode"):
+        dual_calls("cpu")[which]()
+
+
+@gpu
+@pytest.mark.parametrize("which", range(6))
+def test_tangents_are_refused_on_the_gpu(which):
+    with fwAD.dual_level(), pytest.raises(NotImplementedError,
+                                          match="no forward-mode"):
+        dual_calls(DEV)[which]()
+    x, wg, wu = operands(3, bias=False)
+    with fwAD.dual_level(), torch.no_grad(), \
+            pytest.raises(NotImplementedError, match="no forward-mode"):
+        ops.gated_linear(fwAD.make_dual(x[None], x[None]), wg, wu)
+
+
+@gpu
+def test_tangents_of_a_gradient_are_refused():
+    x, wg, wu = [t.requires_grad_() for t in operands(3, bias=False)]
+    for y in (ops.dropout(x, 0.5, 1, 1), ops.gated_linear(x, wg, wu)):
+        dy = torch.ones_like(y)
+        with fwAD.dual_level(), pytest.raises(NotImplementedError,
+                                              match="no forward-mode"):
+            torch.autograd.grad(y, x, fwAD.make_dual(dy, dy))
