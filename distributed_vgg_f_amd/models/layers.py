@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.nn.modules.module import _has_any_global_hook
 
 from .. import ops
 
@@ -49,11 +50,22 @@ class Linear(nn.Module):
         return ops.linear(x, self.weight, self.bias, self.relu)
 
 
+def _only_runs(m: nn.Module, cls: type) -> bool:
+    """Whether a call of m does nothing but cls.forward, so that another layer
+    may do its work for it: no subclass, no hooks, no replaced forward."""
+    return (type(m) is cls and "forward" not in vars(m)
+            and not (m._forward_hooks or m._forward_pre_hooks
+                     or m._backward_hooks or m._backward_pre_hooks)
+            and not _has_any_global_hook())
+
+
 class GatedLinear(nn.Module):
     """act(x @ w_gate + b_gate) * (x @ w_up + b_up), x [M,K], both w [K,N].
 
     With a Dropout layer as second argument its mask is drawn in the same
-    kernel (the layer's counter advances as if it had been called)."""
+    kernel (the layer's counter advances as if it had been called). A layer
+    that is more than that, with hooks or of another type, is called on the
+    result."""
 
     def __init__(self, k: int, n: int, act: str = "silu", bias: bool = True,
                  std: Optional[float] = None):
@@ -70,6 +82,8 @@ class GatedLinear(nn.Module):
 
     def forward(self, x, drop: Optional["Dropout"] = None):
         w = (self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
+        if drop is not None and not _only_runs(drop, Dropout):
+            return drop(ops.gated_linear(x, *w, act=self.act))
         if drop is None or not drop.training or drop.p <= 0.0:
             return ops.gated_linear(x, *w, act=self.act)
         drop._calls += 1
@@ -84,8 +98,10 @@ def hidden_fc(k: int, n: int, gate: str = "") -> nn.Module:
 
 
 def run_hidden(fc: nn.Module, drop: "Dropout", x):
-    """A hidden layer and the dropout behind it."""
-    return fc(x, drop) if isinstance(fc, GatedLinear) else drop(fc(x))
+    """A hidden layer and the dropout behind it, in one if neither has
+    anything attached that looks at what passes between them."""
+    one = _only_runs(fc, GatedLinear) and _only_runs(drop, Dropout)
+    return fc(x, drop) if one else drop(fc(x))
 
 
 class LRN(nn.Module):
