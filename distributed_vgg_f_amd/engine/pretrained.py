@@ -56,12 +56,22 @@ def load_matconvnet_vggf(path: str, model: torch.nn.Module) -> int:
 
     Returns the number of parameter tensors loaded. Unknown layer names are
     skipped (MatConvNet files carry relu/norm/pool layers without weights).
+    A layer that the model has in another form, as the gated fc6 and fc7 of
+    Config.fc_gate, is refused before anything is loaded.
     """
     from scipy.io import loadmat
     mat = loadmat(path, struct_as_record=True, squeeze_me=False)
     params = dict(model.named_parameters())
+    layers = _layers_from_mat(mat)
+    other = sorted({prefix for prefix in
+                    (VGGF_LAYER_MAP.get(layer["name"]) for layer in layers)
+                    if prefix and prefix + ".weight" not in params
+                    and any(n.startswith(prefix + ".") for n in params)})
+    if other:
+        raise ValueError(f"{', '.join(other)}: the model's layers have no "
+                         "weight of the file's form (gated layers?)")
     loaded = 0
-    for layer in _layers_from_mat(mat):
+    for layer in layers:
         prefix = VGGF_LAYER_MAP.get(layer["name"])
         if prefix is None:
             continue

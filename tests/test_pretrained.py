@@ -6,6 +6,7 @@ the weights land in the right VGG-F parameters.
 """
 
 import numpy as np
+import pytest
 import torch
 from scipy.io import savemat
 
@@ -65,3 +66,14 @@ def test_matconvnet_import(tmp_path):
                           torch.from_numpy(cell))
     # fc6 reshaped 6x6x256x4096 -> [9216, 4096]
     assert params["fc6.weight"].shape == (9216, 4096)
+
+
+def test_a_gated_head_is_refused_before_anything_is_loaded(tmp_path):
+    path = str(tmp_path / "imagenet-vgg-f.mat")
+    _synthetic_mat(path)
+    model = build_model(Config(model="vggf", fc_gate="silu"))
+    before = {n: p.detach().clone() for n, p in model.named_parameters()}
+    with pytest.raises(ValueError, match="fc6, fc7: .*no weight"):
+        load_matconvnet_vggf(path, model)
+    for n, p in model.named_parameters():
+        assert torch.equal(p, before[n]), n
