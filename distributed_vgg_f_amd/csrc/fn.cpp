@@ -33,6 +33,16 @@ static void check_memory(const at::Tensor& t, const char* name) {
               "own, no function transforms (vmap, torch.func)");
 }
 
+// t as a kernel may read it: a view that negates (the imaginary part of a
+// conjugate) made real, zeros without memory refused.
+static at::Tensor readable(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!t._is_zerotensor(), name, ": zeros without memory");
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+static OptTensor readable(const OptTensor& t, const char* name) {
+  return t ? OptTensor(readable(*t, name)) : t;
+}
+
 // A tangent would be lost without a word: the kernels do not see it.
 static void check_tangent(const at::Tensor& t, const char* name) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, ": no "
@@ -63,17 +73,19 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
     Variable dx;
     if (grads[0].defined()) {
       check_tangent(grads[0], "dropout");
+      auto dy = readable(grads[0], "dropout");
       dx = at::GradMode::is_enabled()
-               ? DropoutFn::apply(grads[0], p, seed, offset, used)
-               : dropout(grads[0].contiguous(), p, seed, offset, used)[0];
+               ? DropoutFn::apply(dy, p, seed, offset, used)
+               : dropout(dy.contiguous(), p, seed, offset, used)[0];
     }
     return {dx, Variable(), Variable(), Variable(), Variable()};
   }
 };
 
-at::Tensor dropout_ad(const at::Tensor& x, double p, int64_t seed,
+at::Tensor dropout_ad(const at::Tensor& x_, double p, int64_t seed,
                       int64_t offset, const OptTensor& offset_t) {
-  check_tangent(x, "dropout");
+  check_tangent(x_, "dropout");
+  auto x = readable(x_, "dropout");
   if (at::GradMode::is_enabled() && x.requires_grad())
     return DropoutFn::apply(x, p, seed, offset, offset_t);
   return dropout(x.contiguous(), p, seed, offset, offset_t)[0];
@@ -143,7 +155,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     }
     OptTensor used;
     if (s.size() > 4) used = s[4];
-    auto r = gated_bwd(grads[0], s[0], s[1], s[2], s[3], d["K"].toInt(),
+    auto r = gated_bwd(readable(grads[0], "gated_linear"), s[0], s[1], s[2], s[3], d["K"].toInt(),
                        d["N"].toInt(), d["act"].toInt(), d["p"].toDouble(),
                        d["seed"].toInt(), d["offset"].toInt(), used, need,
                        outs);
@@ -156,14 +168,18 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
                                          "bu_out"};
 };
 
-at::Tensor gated_ad(const at::Tensor& x, const at::Tensor& wg,
-                    const at::Tensor& wu, const OptTensor& bg,
-                    const OptTensor& bu, int64_t act, double p, int64_t seed,
+at::Tensor gated_ad(const at::Tensor& x_, const at::Tensor& wg_,
+                    const at::Tensor& wu_, const OptTensor& bg_,
+                    const OptTensor& bu_, int64_t act, double p, int64_t seed,
                     int64_t offset, const OptTensor& offset_t,
                     const OptTensor& wg_grad, const OptTensor& wu_grad,
                     const OptTensor& bg_grad, const OptTensor& bu_grad) {
-  for (auto* t : {&x, &wg, &wu}) check_tangent(*t, "gated_linear");
-  for (auto* t : {&bg, &bu}) if (*t) check_tangent(**t, "gated_linear");
+  const char* name = "gated_linear";
+  for (auto* t : {&x_, &wg_, &wu_}) check_tangent(*t, name);
+  for (auto* t : {&bg_, &bu_}) if (*t) check_tangent(**t, name);
+  auto x = readable(x_, name), wg = readable(wg_, name),
+       wu = readable(wu_, name);
+  auto bg = readable(bg_, name), bu = readable(bu_, name);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || wg.requires_grad() || wu.requires_grad() ||
        (bg && bg->requires_grad()) || (bu && bu->requires_grad())))

@@ -145,3 +145,53 @@ def test_tangents_of_a_gradient_are_refused():
         with fwAD.dual_level(), pytest.raises(NotImplementedError,
                                               match="no forward-mode"):
             torch.autograd.grad(y, x, fwAD.make_dual(dy, dy))
+
+
+@gpu
+def test_views_that_negate():
+    z = torch.randn(40, 48, dtype=torch.complex64, device=DEV)
+    for x in (z.conj().imag, torch._neg_view(z.real.contiguous()),
+              torch._neg_view(z.real.bfloat16())):
+        assert x.is_neg()
+        real = x.clone()
+        want = ops.dropout(real, 0.5, 1, 1)
+        assert torch.equal(ops.dropout(x, 0.5, 1, 1), want)
+        leaf = real.clone().requires_grad_()
+        y = ops.dropout(leaf, 0.5, 1, 1)
+        dx, = torch.autograd.grad(y, leaf, x)
+        assert torch.equal(dx, want)
+    ts = operands(5)
+    h = ops.gated_linear(*ts)
+    for which in range(5):
+        neg = list(ts)
+        neg[which] = torch._neg_view(-ts[which])
+        assert torch.equal(ops.gated_linear(*neg), h)
+    leaf = ts[0].clone().requires_grad_()
+    dh = torch.randn_like(h)
+    got, = torch.autograd.grad(ops.gated_linear(leaf, *ts[1:]), leaf,
+                               torch._neg_view(-dh))
+    want, = torch.autograd.grad(ops.gated_linear(leaf, *ts[1:]), leaf, dh)
+    assert torch.equal(got, want)
+
+
+def zero_calls(dev):
+    ext = ops.native.ext()
+    zero = torch._efficientzerotensor((8, 8), dtype=torch.bfloat16, device=dev)
+    w = torch.ones(8, 8, dtype=torch.bfloat16, device=dev)
+    flat = torch._efficientzerotensor((8,), dtype=torch.bfloat16, device=dev)
+
+    def gated(x=w, g=w, u=w, b=None):
+        return ext.gated_linear(x, g, u, b, None, 0, 0.0, 0, 0, None,
+                                [None] * 4)
+    return [lambda: ext.dropout(zero, 0.5, 1, 1), lambda: gated(x=zero),
+            lambda: gated(g=zero), lambda: gated(u=zero),
+            lambda: gated(b=flat)]
+
+
+@pytest.mark.skipif(not ops.native.available(),
+                    reason="needs the built extension")
+@pytest.mark.parametrize("which", range(5))
+def test_zeros_without_memory_are_refused(which):
+    # on the CPU: the refusal comes before anything is asked of a GPU
+    with pytest.raises(RuntimeError, match="zeros without memory"):
+        zero_calls("cpu")[which]()
