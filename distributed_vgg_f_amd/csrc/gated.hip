@@ -93,10 +93,13 @@ DEV f32x8 act8(int act, f32x8 g, f32x8& d) {
         return v * s;
       });
     case SIGMOID:
+      // s' = e / (1 + e)^2 with e = exp(-|g|): s (1 - s) would cancel where s
+      // is near 1, by 1 % at 12
       return each(g, [&](float v, int r) {
-        float s = sigmoid_f(v);
-        d[r] = s * (1.f - s);
-        return s;
+        float e = __expf(-__builtin_fabsf(v));
+        float s = __builtin_amdgcn_rcpf(1.f + e);
+        d[r] = e * s * s;
+        return v < 0.f ? e * s : s;
       });
     default:
       return each(g, [&](float v, int r) {

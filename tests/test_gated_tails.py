@@ -36,7 +36,7 @@ def exact(act, g):
     if act == "relu":
         return g.clamp(min=0), (g > 0).double()
     s, t = torch.sigmoid(g), torch.sigmoid(-g)
-    return g * s, s * (1 + g * t)
+    return (s, s * t) if act == "sigmoid" else (g * s, s * (1 + g * t))
 
 
 def errors(act, g):
@@ -59,14 +59,16 @@ def errors(act, g):
             2 * rel * (s + a * s * (1 - s) * dz) + \
             (4 * E * s + FLUSH) * (1 + a * dz)
     rel = (2 * a + 8) * E
-    assert act == "silu"
+    if act == "sigmoid":
+        return rel * s + FLUSH, 2 * rel * s * (1 - s) + FLUSH
     return (rel * s + FLUSH) * a, 2 * rel * (s + a * s * (1 - s)) + \
         (4 * E * s + FLUSH) * (1 + a)
 
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu",
+                                 "sigmoid"])
 def test_values_and_derivatives(act, dtype):
     e = torch.finfo(dtype).eps / 2
     least = torch.finfo(dtype).smallest_normal * e
