@@ -1041,6 +1041,16 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
   return best;
 }
 
+// What make_plan chooses, for tests that want every tile: fm, fn, bk, ring,
+// brief, splits. product: 0 forward, 1 dX, 2 weight gradients.
+std::vector<int64_t> gated_plan(int64_t product, int64_t rows, int64_t cols,
+                                int64_t k_len) {
+  TORCH_CHECK(product >= FWD && product <= WGRAD && rows > 0 && cols > 0 &&
+              k_len > 0, "gated_plan: no such product");
+  const Plan p = make_plan(int(product), rows, cols, k_len);
+  return {p.fm, p.fn, p.bk, p.ring, p.brief, p.splits};
+}
+
 template <class T, int MODE>
 static void launch(const Plan& pl, const ProductArgs& a) {
   dim3 grid(u32(pl.tiles_m) * pl.tiles_n * pl.splits);

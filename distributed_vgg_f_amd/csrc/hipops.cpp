@@ -44,6 +44,9 @@ at::Tensor gated_call(const at::Tensor&, const at::Tensor&, const at::Tensor&,
                       int64_t, int64_t, const c10::optional<at::Tensor>&,
                       const std::vector<c10::optional<at::Tensor>>&);
 
+// gated.hip
+std::vector<int64_t> gated_plan(int64_t, int64_t, int64_t, int64_t);
+
 // lrnpool.hip
 at::Tensor lrn_fwd(const at::Tensor&, int64_t, double, double, double);
 at::Tensor lrn_bwd(const at::Tensor&, const at::Tensor&, int64_t, double,
@@ -102,6 +105,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("w_up"), py::arg("bias_gate"), py::arg("bias_up"),
         py::arg("act"), py::arg("p"), py::arg("seed"), py::arg("offset"),
         py::arg("offset_t"), py::arg("grad_outs"));
+  m.def("gated_plan", &dvgg::gated_plan, py::arg("product"),
+        py::arg("rows"), py::arg("cols"), py::arg("k_len"));
   m.def("lrn_fwd", &dvgg::lrn_fwd);
   m.def("lrn_bwd", &dvgg::lrn_bwd);
   m.def("maxpool_fwd", &dvgg::maxpool_fwd);
