@@ -1234,6 +1234,7 @@ std::vector<at::Tensor> gated_fwd(
     hipLaunchKernelGGL(copy_offset_kernel, dim3(1), dim3(1), 0, cur_stream(),
                        d.offset_ptr,
                        reinterpret_cast<i64*>(used.data_ptr<int64_t>()));
+    HIP_CHECK(hipGetLastError());
   }
   at::Tensor ops_[3] = {x, wg, wu};
   at::Tensor &xl = ops_[0], &gl = ops_[1], &ul = ops_[2];
