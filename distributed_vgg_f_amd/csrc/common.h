@@ -37,6 +37,17 @@ DEV u16 f2bf(float f) {
   return u16((u + round) >> 16);
 }
 
+// both 16-bit types, named by a value of the type. from_f: one v_cvt_pk for
+// two; round to nearest even, as f2bf
+DEV float to_f(u16 v, __bf16) { return bf2f(v); }
+DEV float to_f(u16 v, _Float16) {
+  return float(__builtin_bit_cast(_Float16, v));
+}
+DEV u16 from_f(float v, __bf16) { return __builtin_bit_cast(u16, __bf16(v)); }
+DEV u16 from_f(float v, _Float16) {
+  return __builtin_bit_cast(u16, _Float16(v));
+}
+
 DEV f32x2 bf2x2(u32 packed) {
   f32x2 r;
   r.x = bf2f(u16(packed & 0xffffu));

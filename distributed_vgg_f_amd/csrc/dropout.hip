@@ -20,15 +20,6 @@ static inline hipStream_t cur_stream() {
   return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
 }
 
-DEV float to_f(u16 v, __bf16) { return bf2f(v); }
-DEV float to_f(u16 v, _Float16) {
-  return float(__builtin_bit_cast(_Float16, v));
-}
-DEV u16 from_f(float v, __bf16) { return f2bf(v); }
-DEV u16 from_f(float v, _Float16) {
-  return __builtin_bit_cast(u16, _Float16(v));
-}
-
 // 16-bit types: 8 elements (two blocks of the generator) a lane and step.
 template <class T>
 __global__ __launch_bounds__(256) void dropout16_kernel(

@@ -30,16 +30,6 @@ static inline hipStream_t cur_stream() {
   return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
 }
 
-DEV float to_f(u16 v, __bf16) { return bf2f(v); }
-DEV float to_f(u16 v, _Float16) {
-  return float(__builtin_bit_cast(_Float16, v));
-}
-// one v_cvt_pk for two; round to nearest even, as f2bf
-DEV u16 from_f(float v, __bf16) { return __builtin_bit_cast(u16, __bf16(v)); }
-DEV u16 from_f(float v, _Float16) {
-  return __builtin_bit_cast(u16, _Float16(v));
-}
-
 // ------------------------------------------------------------- activations
 enum Act { SILU, GELU, GELU_TANH, RELU, SIGMOID };
 

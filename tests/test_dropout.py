@@ -275,3 +275,21 @@ def test_layer_draws_a_new_mask_at_each_call():
     check(b, x.cpu(), 0.5, 3, 2)
     layer.eval()
     assert layer(x) is x
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_value_of_16_bits(dtype):
+    # subnormal numbers, infinities and NaN among them, and products that
+    # overflow or fall into the subnormal range
+    bits = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16)
+    x = bits.view(dtype).to(DEV)
+    for p in (0.5, 0.3, 0.999):
+        y = ops.dropout(x, p, 1, 1).cpu()
+        keep = keep_mask(x.shape, p, 1, 1)
+        scale = torch.tensor(1 / (1 - p), dtype=torch.float32)
+        want = torch.where(keep, x.cpu().float() * scale, 0.0).to(dtype)
+        nan = torch.isnan(want)
+        assert torch.equal(torch.isnan(y), nan)
+        assert torch.equal(y[~nan].view(torch.int16),
+                           want[~nan].view(torch.int16))
