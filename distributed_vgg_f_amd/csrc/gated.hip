@@ -215,7 +215,8 @@ DEV void finish8(const OutArgs& o, u32 off, int m, int n, f32x8 g, f32x8 u) {
 // ---------------------------------------------------------------- products
 // FWD    [M][2N] = X [Wg | Wu]             a tile: 16 FN columns of each
 // DGRAD  [M][K]  = dG Wg^T + dU Wu^T       two parts of the contraction
-// WGRAD  2 x [K][N] = X^T dG, X^T dU       a tile lies in one of the two
+// WGRAD  2 x [K][N] = X^T dG, X^T dU       a tile lies in one of the two; or
+//                                          one of them alone
 enum Mode { FWD, DGRAD, WGRAD };
 
 struct ProductArgs {
@@ -226,7 +227,8 @@ struct ProductArgs {
   int k_len;
   int splits;
   int tiles_m, tiles_n;
-  float* slab;          // [splits][2 or 1][rows][slab_ld] if splits > 1
+  int mats;             // output matrices: FWD 2, DGRAD 1, WGRAD either
+  float* slab;          // [splits][mats][rows][slab_ld] if splits > 1
   i64 slab_ld;          // cols rounded up to 8
   u16* c[2];            // outputs of DGRAD ([0]) and WGRAD
   OutArgs out;          // of FWD
@@ -290,8 +292,8 @@ void product_kernel(ProductArgs p) {
   t %= group;
   const int m0 = __builtin_amdgcn_readfirstlane((g0 + t % gs) * TL::BM);
   int tn = __builtin_amdgcn_readfirstlane(t / gs);
-  // WGRAD: the second half of the tile columns belongs to dU
-  const int which = MODE == WGRAD && tn >= p.tiles_n / 2;
+  // WGRAD of both: the second half of the tile columns belongs to dU
+  const int which = MODE == WGRAD && p.mats == 2 && tn >= p.tiles_n / 2;
   if (which) tn -= p.tiles_n / 2;
   const int n0 = tn * (MODE == FWD ? TL::HALF : TL::BN);
 
@@ -339,7 +341,6 @@ void product_kernel(ProductArgs p) {
   const int mw = m0 + (wave >> 1) * 16 * FM + c;
   const int wide = 16 * (q & 1) + 8 * (q >> 1);
   if constexpr (MODE != FWD) {
-    constexpr int MATS = MODE == WGRAD ? 2 : 1;
     const int nw = n0 + (wave & 1) * TL::HALF;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -355,7 +356,7 @@ void product_kernel(ProductArgs p) {
         }
       } else {
         float* o = p.slab +
-            (((i64)split * MATS + which) * p.rows + m) * p.slab_ld;
+            (((i64)split * p.mats + which) * p.rows + m) * p.slab_ld;
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
           const int n = nw + 16 * j + 4 * q;
@@ -968,7 +969,7 @@ struct Plan { int fm, fn, bk, ring, splits, tiles_m, tiles_n; bool brief; };
 // 0.38; 2048 x 4096 x 1000: 51.4 -> 39.2, 512 x 4096 x 4096: 54.3 -> 46.3).
 // Two tiles on a CU cover for each other, and then two buffers each are the
 // faster (797 x 5368 x 3032: 91 us, with four buffers 107).
-static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
+static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len, int mats) {
   struct Kind {
     int fm, fn, bk, ring, per_cu;
     double one, all, edge;
@@ -983,11 +984,11 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
                                {4, 4, 64, 2, 4, 0.69, 1.85, 3.9, true}};
   constexpr double CUS = 256, MEM = 4.5e6, JOIN_MEM = 7e6;
   const double join = mode == FWD ? 4.0 : 2.4;
-  const double mats = mode == DGRAD ? 1 : 2;
   const double out = double(rows) * cols;
   // bytes that the product moves at least
   const double ab = mode == FWD ? rows + 2. * cols
-                  : mode == DGRAD ? 2. * rows + 2. * cols : rows + 2. * cols;
+                  : mode == DGRAD ? 2. * rows + 2. * cols
+                                  : rows + double(mats) * cols;
   const double mem = 2 * (ab * k_len + (mode == FWD ? 3 : mats) * out) / MEM;
   Plan best{};
   double least = 0;
@@ -1001,7 +1002,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
     if (k.brief && (mode != WGRAD || k_len > 64)) continue;
     const int tm = ceil_div(rows, 32 * k.fm);
     const int tn = ceil_div(cols, (mode == FWD ? 16 : 32) * k.fn) *
-                   (mode == WGRAD ? 2 : 1);
+                   (mode == WGRAD ? mats : 1);
     // turns of the loop: a stage in each buffer (of 64 k: stages of 32 k come
     // two at a time), of DGRAD's two parts in turns
     const int turns = ceil_div(k_len, 64 * k.ring / (mode == DGRAD ? 2 : 1));
@@ -1021,7 +1022,7 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
       const double full = std::floor(wgs / slots);
       double t = full * round(slots) + round(wgs - full * slots);
       t = std::sqrt(std::sqrt(t * t * t * t + mem * mem * mem * mem));
-      if (sp > 1) t += join + sp * mats * out * 8 / JOIN_MEM;
+      if (sp > 1) t += join + double(sp) * mats * out * 8 / JOIN_MEM;
       if (least == 0 || t < least) {
         least = t;
         best = Plan{k.fm, k.fn, k.bk, k.ring, sp, tm, tn, k.brief};
@@ -1032,12 +1033,13 @@ static Plan make_plan(int mode, i64 rows, i64 cols, i64 k_len) {
 }
 
 // What make_plan chooses, for tests that want every tile: fm, fn, bk, ring,
-// brief, splits. product: 0 forward, 1 dX, 2 weight gradients.
+// brief, splits. product: 0 forward, 1 dX, 2 both weight gradients, 3 one.
 std::vector<int64_t> gated_plan(int64_t product, int64_t rows, int64_t cols,
                                 int64_t k_len) {
-  TORCH_CHECK(product >= FWD && product <= WGRAD && rows > 0 && cols > 0 &&
+  TORCH_CHECK(product >= FWD && product <= WGRAD + 1 && rows > 0 && cols > 0 &&
               k_len > 0, "gated_plan: no such product");
-  const Plan p = make_plan(int(product), rows, cols, k_len);
+  const Plan p = make_plan(int(std::min<int64_t>(product, WGRAD)), rows, cols,
+                           k_len, product % 2 ? 1 : 2);
   return {p.fm, p.fn, p.bk, p.ring, p.brief, p.splits};
 }
 
@@ -1089,16 +1091,16 @@ static void join_gated(bool half, const float* slab, int splits, i64 slab_ld,
 }
 
 template <int MODE>
-static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
+static void product(at::ScalarType type, ProductArgs& a,
                     const at::TensorOptions& opt) {
+  const Plan pl = make_plan(MODE, a.rows, a.cols, a.k_len, a.mats);
   a.splits = pl.splits;
   a.tiles_m = pl.tiles_m;
   a.tiles_n = pl.tiles_n;
   a.slab_ld = up(a.cols, 8);
-  const int mats = MODE == DGRAD ? 1 : 2;
   at::Tensor slab;
   if (pl.splits > 1) {
-    slab = at::empty({(i64)pl.splits * mats * a.rows * a.slab_ld},
+    slab = at::empty({(i64)pl.splits * a.mats * a.rows * a.slab_ld},
                      opt.dtype(at::kFloat));
     a.slab = slab.data_ptr<float>();
   }
@@ -1110,16 +1112,16 @@ static void product(at::ScalarType type, const Plan& pl, ProductArgs& a,
     join_gated(half, a.slab, pl.splits, a.slab_ld, a.out);
     return;
   }
-  i64 chunks = (i64)a.rows * (MODE == WGRAD ? 2 : 1) * a.slab_ld / 8;
+  i64 chunks = (i64)a.rows * a.mats * a.slab_ld / 8;
   dim3 grid(u32(std::min<i64>((chunks + 255) / 256, 8192)));
   auto st = cur_stream();
   if (half) {
     hipLaunchKernelGGL(join_plain_kernel<_Float16>, grid, dim3(256), 0, st,
-                       a.slab, pl.splits, a.slab_ld, a.rows, a.cols, mats,
+                       a.slab, pl.splits, a.slab_ld, a.rows, a.cols, a.mats,
                        a.c[0], a.c[1]);
   } else {
     hipLaunchKernelGGL(join_plain_kernel<__bf16>, grid, dim3(256), 0, st,
-                       a.slab, pl.splits, a.slab_ld, a.rows, a.cols, mats,
+                       a.slab, pl.splits, a.slab_ld, a.rows, a.cols, a.mats,
                        a.c[0], a.c[1]);
   }
   HIP_CHECK(hipGetLastError());
@@ -1252,11 +1254,12 @@ std::vector<at::Tensor> gated_fwd(
     a.rows = int(M);
     a.cols = int(N);
     a.k_len = int(K);
+    a.mats = 2;
     a.out = OutArgs{mptr(h), train ? gu.data_ptr<float>() : nullptr,
                     {bg ? cptr(bgc) : nullptr, bu ? cptr(buc) : nullptr},
                     int(M), int(N), ldg, int(act), p > 0.0, d};
     if (M <= ROWS_MAX) product_rows(type, a, any, x.options());
-    else product<FWD>(type, make_plan(FWD, M, N, K), a, x.options());
+    else product<FWD>(type, a, x.options());
   }
   if (!train) return {h};
   std::vector<at::Tensor> r{h, gu, xl, gl, ul};
@@ -1361,25 +1364,25 @@ std::vector<at::Tensor> gated_bwd(
       q.rows = int(M);
       q.cols = int(K);
       q.k_len = int(N);
+      q.mats = 1;
       q.c[0] = ptr(0);
-      product<DGRAD>(type, make_plan(DGRAD, M, K, N), q, opt);
+      product<DGRAD>(type, q, opt);
     }
     if (need & 6) {
-      // one of the two alone: the other is computed beside it
-      at::Tensor spare;
-      if ((need & 6) != 6) spare = at::empty({K, N}, opt);
+      const bool gate = need & 2, both = (need & 6) == 6;
       ProductArgs q{};
       q.a[0] = q.a[1] = cptr(x);
-      q.b[0] = dg;
-      q.b[1] = du;
+      q.b[0] = gate ? dg : du;
+      q.b[1] = both ? du : nullptr;
       q.lda = ld_of(x);
       q.ldb = ldg;
       q.rows = int(K);
       q.cols = int(N);
       q.k_len = int(M);
-      q.c[0] = need & 2 ? ptr(1) : mptr(spare);
-      q.c[1] = need & 4 ? ptr(2) : mptr(spare);
-      product<WGRAD>(type, make_plan(WGRAD, K, N, M), q, opt);
+      q.mats = both ? 2 : 1;
+      q.c[0] = ptr(gate ? 1 : 2);
+      q.c[1] = both ? ptr(2) : nullptr;
+      product<WGRAD>(type, q, opt);
     }
   }
   for (int i = 0; i < 5; ++i)
