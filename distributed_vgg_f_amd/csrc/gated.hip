@@ -83,13 +83,12 @@ DEV f32x8 act8(int act, f32x8 g, f32x8& d) {
         return v * s;
       });
     case SIGMOID:
-      // s' = e / (1 + e)^2 with e = exp(-|g|): s (1 - s) would cancel where s
-      // is near 1, by 1 % at 12
+      // s' = e / (1 + e)^2 with e = exp(-g): s (1 - s) would cancel where s
+      // is near 1, by 0.5 % at 12. Past 1e38 s is 0, and e may be infinite.
       return each(g, [&](float v, int r) {
-        float e = __expf(-__builtin_fabsf(v));
-        float s = __builtin_amdgcn_rcpf(1.f + e);
-        d[r] = e * s * s;
-        return v < 0.f ? e * s : s;
+        float e = __expf(-v), s = __builtin_amdgcn_rcpf(1.f + e);
+        d[r] = __builtin_fminf(e, 1e38f) * s * s;
+        return s;
       });
     default:
       return each(g, [&](float v, int r) {

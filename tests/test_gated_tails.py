@@ -104,3 +104,30 @@ def test_values_and_derivatives(act, dtype):
         err[G == 0] = 2.0 ** 15                     # either side of the border
     bad = ~(off <= err)
     assert not bool(bad.any()), G[bad].tolist()
+
+
+@gpu
+def test_infinite_gates():
+    inf, nan = float("inf"), float("nan")
+    b = torch.tensor([inf, -inf, nan, 1e4, -1e4], dtype=torch.bfloat16)
+    x, w = torch.ones(20, 1), torch.zeros(1, 5)
+    ts = [t.bfloat16().to(DEV) for t in (x, w, w, b, torch.full((5,), 2.0))]
+
+    def run(act):
+        leaf = ts[3].detach().requires_grad_()
+        h = ops.gated_linear(*ts[:3], leaf, ts[4], act=act)
+        db, = torch.autograd.grad(h, leaf, torch.ones_like(h))
+        return h.detach()[0].cpu().float(), db.cpu().float()
+    h, db = run("sigmoid")
+    assert h[[0, 1, 3, 4]].tolist() == [2, 0, 2, 0]
+    assert db[[0, 1, 3, 4]].tolist() == [0, 0, 0, 0]
+    h, db = run("relu")
+    assert h[:2].tolist() == [inf, 0] and db[[0, 1, 3, 4]].tolist() == [40, 0,
+                                                                       40, 0]
+    for act in ("silu", "gelu", "gelu_tanh", "relu", "sigmoid"):
+        h, db = run(act)
+        assert math.isnan(h[2])
+        assert act == "relu" or math.isnan(db[2])
+        if act not in ("sigmoid", "relu"):        # g and 0, and slopes 1 and 0
+            assert h[0] == inf and h[3:].tolist() == [2 * float(b[3]), 0]
+            assert db[3:].tolist() == [40, 0]
