@@ -195,3 +195,19 @@ def test_zeros_without_memory_are_refused(which):
     # on the CPU: the refusal comes before anything is asked of a GPU
     with pytest.raises(RuntimeError, match="zeros without memory"):
         zero_calls("cpu")[which]()
+
+
+@gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_calls(backend):
+    x, wg, wu = operands(6, bias=False)
+
+    def f(t):
+        return ops.dropout(ops.gated_linear(t, wg, wu) * 2, 0.5, 1, 1) + 1
+    torch._dynamo.reset()
+    a, b = [x.clone().requires_grad_() for _ in range(2)]
+    y, want = torch.compile(f, backend=backend)(a), f(b)
+    assert torch.equal(y, want)
+    y.sum().backward()
+    want.sum().backward()
+    assert torch.equal(a.grad, b.grad)
