@@ -16,7 +16,9 @@
 // nearly double the error of the gradients (bf16, 256 x 9216 x 4096: 0.0031
 // of their size instead of 0.0024, one rounding of the result being 0.0017),
 // and they are 3 to 4 % of the time at the largest sizes, less elsewhere. dG and
-// dU are rounded to the type of x, which the matrix instructions take.
+// dU are rounded to the type of x, which the matrix instructions take; that is
+// all of the difference between the 0.0024 and the 0.0017. Gradients are
+// rounded to the type of x whatever the type of the buffer that they go to.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -254,15 +256,16 @@ DEV s16x8 trade(f32x4 a, f32x4 b) {
 }
 
 // The tiles by rule: make_plan() below. At 8192 x 4096 x 8192 in bf16, each
-// product 1.1 TFLOP: forward 0.95 ms (1.16 PFLOP/s; 0.64 GB leave it, G and U
-// among them), dX 0.88 (1.25), both weights 0.84 (1.31), all of 256 x 256
-// tiles with the matrix cores busy for 70 % of the cycles. What bounds it
-// there is power: the more of them are busy, the lower the clock (1.75 GHz),
-// and 32x32x16 products took 917 and 970 us in place of 840 and 876. At 256 x
-// 9216 x 4096 the forward product takes 59 us, joined in 8, for 151 MB of
-// weights and 17 of slabs (with weights that the last-level cache holds 43):
-// memory, at 2.9 TB/s, though wider reads of the weights (tiles of 64 x 256)
-// took 73.
+// product 1.1 TFLOP: forward 0.96 ms (1.15 PFLOP/s; 0.67 GB leave it, G and U
+// among them), dX 0.87 (1.27), both weights 0.81 (1.36), all of 256 x 256
+// tiles with the matrix cores busy for 60, 66 and 73 % of the cycles. What
+// bounds it there is power: the clock falls to 1.9 GHz, of the 2.4 that short
+// kernels run at, and 32x32x16 products took 917 and 970 us in place of 840
+// and 876. At 256 x 9216 x 4096 the forward product takes 60 us, joined in 2,
+// for 151 MB of weights and 17 of slabs (with weights that the last-level cache
+// holds 43). That is 2.9 TB/s, where rows_kernel streams such weights at 5.1:
+// no limit of the memory but of loads and products that wait for each other;
+// wider reads of the weights (tiles of 64 x 256) took 73.
 template <class T, int MODE, int FM, int FN, int BK, int RING,
           bool SHORT = false>
 __global__ __launch_bounds__(256, SHORT || BK * RING == 64 ? 4
@@ -508,8 +511,8 @@ void product_kernel(ProductArgs p) {
 
 // ------------------------------------------------- joining a split product
 // Sums the slabs in a fixed order (the same result every time; atomics would
-// not give that). 256 x 4096 of a contraction in 8 parts: 67 MB in 11 us, out
-// of the caches that they were just written to. 8 columns a
+// not give that). 256 x 4096 of a contraction in 2 parts: 17 MB read and 10
+// written in 8.5 us, out of the caches that they were just written to. 8 columns a
 // thread; WIDE, for few columns and many slabs: 8 threads, each an eighth of
 // the slabs (one row of 25088 x 64 in 49 slabs: 21.5 -> 9.3 us
 // with its product).
@@ -579,7 +582,7 @@ __global__ __launch_bounds__(256) void join_plain_kernel(
 // columns 8 c .. 8 c + 7. Eight rows of eight columns are turned over by
 // v_perm into eight fragments, one for each column j of the eight, of which
 // lane (c, q) holds column 8 c + j and its 8 k: what the matrix instruction
-// takes. The next 32 k are on their way meanwhile (32 KB a wave). The four
+// takes. The next 32 k are on their way meanwhile (16 KB a wave). The four
 // waves of a block, each with its part of the contraction, meet in LDS; parts
 // of several blocks meet in join_gated_kernel. (With the fragments of 32 or 64
 // rows the tiles are faster: 64 x 25088 x 4096 in 91 us, this way in 112.)
@@ -958,9 +961,11 @@ struct Plan { int fm, fn, bk, ring, splits, tiles_m, tiles_n; bool brief; };
 
 // Which tile, and into how many parts the contraction is split: the least
 // time by a model of what the tiles measured over the 138 products of 46
-// shapes of 17 to 8192 rows and 64 to 25088 columns (it is off by 13 % there;
-// what it picks is 1.5 % slower than the best of all tiles and splits in the
-// mean, 10 % at worst).
+// shapes of 17 to 8192 rows and 64 to 25088 columns. It ranks them: what it
+// picks there is 1.5 % slower than the best of all tiles and splits in the
+// mean, 10 % at worst. Its times are off by 13 % in the mean, and low where
+// the clock falls (forward at 8192 x 4096 x 8192: 714 us for 959) and at
+// ragged widths, for which it has no term (1003 x 1001 x 2747: 18 for 30).
 // Microseconds. A stage costs `one` if a tile has its CU to itself and `all`
 // if the CU is full; `edge` is a tile's first loads and its epilogue.
 // Four buffers are for launches of about one tile a CU: two leave such a tile

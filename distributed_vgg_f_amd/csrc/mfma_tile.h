@@ -47,7 +47,8 @@ DEV void mfma32<_Float16>(f32x4& c, s16x8 a, s16x8 b) {
   asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0"
                : "+a"(c) : "v"(a), "v"(b));
 }
-// 8 passes: 11 wait states before another instruction may touch the result
+// 11 wait states before another instruction may touch the result; behind its
+// own builtin the compiler leaves 8
 DEV void mfma_wait() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 10");

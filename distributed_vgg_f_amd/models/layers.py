@@ -128,8 +128,10 @@ class Dropout(nn.Module):
     """Counter-based dropout: offset advances per call so steps decorrelate.
 
     The counter is the host's, so a captured graph would replay one mask; the
-    trainer runs such models eagerly. ops.dropout and ops.gated_linear also
-    take the offset from the device."""
+    trainer runs such models eagerly. A forward pass that is run again for its
+    backward pass (activation checkpointing) counts again and draws another
+    mask. ops.dropout and ops.gated_linear take the offset from the caller,
+    and from the device."""
 
     def __init__(self, p: float, seed: int = 0):
         super().__init__()

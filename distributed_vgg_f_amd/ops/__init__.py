@@ -43,10 +43,11 @@ def gated_linear(x, w_gate, w_up, bias_gate=None, bias_up=None,
     offset are those of `dropout`, which draws the same mask from them; p = 0
     leaves it out.
 
-    GPU: bf16 or fp16, one type and one device for all operands, any K, N
-    and strides; sums in 32 bits. Operands whose rows do not start on 16
-    bytes are copied to rows that do, once a call (not for answers of up to
-    16 rows). Differentiates once.
+    GPU: bf16 or fp16, one type and one device for all operands, K and N from
+    1 to 2^21, any strides; sums in 32 bits. Operands whose rows do not start
+    on 16 bytes are copied to rows that do, once a call (not for answers of up
+    to 16 rows). Differentiates once, backward; no tangents and no function
+    transforms. A traced call replays the operator.
     """
     if act not in _ACT_ID:
         raise ValueError(f"gated_linear: unknown activation {act!r}; have "
@@ -95,7 +96,10 @@ def dropout(x, p: float, seed: int = 0, offset: Union[int, torch.Tensor] = 0,
     never stored; a dropped element is 0 whatever x holds there. seed and
     offset count modulo 2^32. offset may be one int64 on x's device: a
     captured graph then draws a new mask at each replay if the caller counts
-    it up. CPU: the mask is torch's own, or the one that is given (`mask` is
+    it up. Differentiates backward, any number of times; no tangents and no
+    function transforms; a traced call replays the operator, with the seed and
+    the offset of the recording (an offset on the device is read anew). CPU:
+    the mask is torch's own, or the one that is given (`mask` is
     not read on the GPU).
     """
     if p <= 0.0:
