@@ -34,9 +34,12 @@ static void check_memory(const at::Tensor& t, const char* name) {
 }
 
 // t as a kernel may read it: a view that negates (the imaginary part of a
-// conjugate) made real, zeros without memory refused.
+// conjugate) made real; what has no memory is refused: torch's zeros that are
+// never stored, tensor types that wrap others, storage that was freed.
 static at::Tensor readable(const at::Tensor& t, const char* name) {
   TORCH_CHECK(!t._is_zerotensor(), name, ": zeros without memory");
+  TORCH_CHECK(t.numel() == 0 || t.const_data_ptr(), name, ": a tensor without "
+              "memory");
   return t.is_neg() ? t.resolve_neg() : t;
 }
 static OptTensor readable(const OptTensor& t, const char* name) {
@@ -66,7 +69,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     auto saved = ctx->get_saved_variables();
     OptTensor used;
-    if (!saved.empty()) used = saved[0];
+    if (!saved.empty()) used = readable(saved[0], "dropout");
     const double p = ctx->saved_data["p"].toDouble();
     const int64_t seed = ctx->saved_data["seed"].toInt();
     const int64_t offset = ctx->saved_data["offset"].toInt();
@@ -83,8 +86,9 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
 };
 
 at::Tensor dropout_ad(const at::Tensor& x_, double p, int64_t seed,
-                      int64_t offset, const OptTensor& offset_t) {
+                      int64_t offset, const OptTensor& offset_t_) {
   check_tangent(x_, "dropout");
+  auto offset_t = readable(offset_t_, "dropout");
   auto x = readable(x_, "dropout");
   if (at::GradMode::is_enabled() && x.requires_grad())
     return DropoutFn::apply(x, p, seed, offset, offset_t);
@@ -148,6 +152,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     variable_list result(11);
     if (!grads[0].defined()) return result;
     check_tangent(grads[0], "gated_linear");
+    for (auto& t : s) readable(t, "gated_linear");   // freed meanwhile?
     std::vector<OptTensor> outs(5);
     for (int i = 0; i < 4; ++i) {
       auto it = d.find(OUT[i]);
@@ -171,7 +176,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
 at::Tensor gated_ad(const at::Tensor& x_, const at::Tensor& wg_,
                     const at::Tensor& wu_, const OptTensor& bg_,
                     const OptTensor& bu_, int64_t act, double p, int64_t seed,
-                    int64_t offset, const OptTensor& offset_t,
+                    int64_t offset, const OptTensor& offset_t_,
                     const OptTensor& wg_grad, const OptTensor& wu_grad,
                     const OptTensor& bg_grad, const OptTensor& bu_grad) {
   const char* name = "gated_linear";
@@ -179,7 +184,8 @@ at::Tensor gated_ad(const at::Tensor& x_, const at::Tensor& wg_,
   for (auto* t : {&bg_, &bu_}) if (*t) check_tangent(**t, name);
   auto x = readable(x_, name), wg = readable(wg_, name),
        wu = readable(wu_, name);
-  auto bg = readable(bg_, name), bu = readable(bu_, name);
+  auto bg = readable(bg_, name), bu = readable(bu_, name),
+       offset_t = readable(offset_t_, name);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || wg.requires_grad() || wu.requires_grad() ||
        (bg && bg->requires_grad()) || (bu && bu->requires_grad())))

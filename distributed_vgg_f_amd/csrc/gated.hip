@@ -1295,7 +1295,8 @@ std::vector<at::Tensor> gated_bwd(
     auto& out = outs[i];
     if (out)
       TORCH_CHECK(out->is_contiguous() && out->device() == x.device() &&
-                  out->numel() == shapes[i][0] * shapes[i][1],
+                  out->numel() == shapes[i][0] * shapes[i][1] &&
+                  out->const_data_ptr(),
                   "gated_linear: bad gradient buffer");
     // a buffer of another type, or one that vectors do not fit, is filled by
     // a copy at the end

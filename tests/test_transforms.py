@@ -211,3 +211,69 @@ def test_compiled_calls(backend):
     y.sum().backward()
     want.sum().backward()
     assert torch.equal(a.grad, b.grad)
+
+
+class Wrapped(torch.Tensor):
+    """A tensor type whose memory is another tensor's."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+def freed(t):
+    t = t.clone()
+    t.untyped_storage().resize_(0)
+    return t
+
+
+@pytest.mark.skipif(not ops.native.available(),
+                    reason="needs the built extension")
+@pytest.mark.parametrize("make", [Wrapped, freed])
+@pytest.mark.parametrize("which", range(8))
+def test_tensors_without_memory_are_refused(which, make):
+    # on the CPU: the refusal comes before anything is asked of a GPU
+    ext = ops.native.ext()
+    w, b = torch.ones(8, 8).bfloat16(), torch.ones(8).bfloat16()
+    ts = [w, w.clone(), w.clone(), b, b.clone(), torch.zeros(1).long()]
+    if which < 6:
+        ts[which] = make(ts[which])
+
+    def call():
+        if which == 6:
+            return ext.dropout(make(w), 0.5, 1, 0)
+        if which == 7:
+            return ext.dropout(w, 0.5, 1, 0, make(ts[5]))
+        return ext.gated_linear(*ts[:5], 0, 0.5, 0, 0, ts[5], [None] * 4)
+    with pytest.raises(RuntimeError, match="without memory"):
+        call()
+
+
+@gpu
+def test_memory_freed_before_the_backward_pass_is_refused():
+    x, wg, wu = operands(6, bias=False)
+    wg.requires_grad_()
+    h = ops.gated_linear(x, wg, wu)
+    x.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="without memory"):
+        h.backward(torch.ones_like(h))
+    x = operands(6, bias=False)[0]
+    wg._dvgg_gbuf = torch.empty_like(wg)
+    h = ops.gated_linear(x, wg, wu)
+    wg._dvgg_gbuf.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="bad gradient buffer"):
+        h.backward(torch.ones_like(h))
+
+
+@gpu
+def test_calls_under_autocast():
+    x, wg, wu = operands(6, bias=False)
+    with torch.autocast("cuda", torch.float16):
+        y, h = ops.dropout(x, 0.5, 1, 1), ops.gated_linear(x, wg, wu)
+    assert torch.equal(y, ops.dropout(x, 0.5, 1, 1))
+    assert torch.equal(h, ops.gated_linear(x, wg, wu))
