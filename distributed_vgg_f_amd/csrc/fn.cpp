@@ -109,6 +109,17 @@ at::Tensor dropout_call(const at::Tensor& x, double p, int64_t seed,
   return op.call(x, p, seed, offset, offset_t);
 }
 
+// The arena's buffer for a weight's gradient, the attribute that ArenaOptimizer
+// gives it. Looked up here and not passed in: a recorded call would hold the
+// buffers as constants, and constants of equal values become one.
+static OptTensor grad_buffer(const OptTensor& t) {
+  if (!t || !t->requires_grad()) return {};
+  py::gil_scoped_acquire gil;
+  py::object buffer = py::getattr(py::cast(*t), "_dvgg_gbuf", py::none());
+  if (buffer.is_none()) return {};
+  return buffer.cast<at::Tensor>();
+}
+
 // Keeps both projections; backward is one pass over them and two products.
 // *_out: gradient buffers of the engine's arena, written in place. What is
 // returned for them is a fresh view: AccumulateGrad stores a gradient only
@@ -176,9 +187,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
 at::Tensor gated_ad(const at::Tensor& x_, const at::Tensor& wg_,
                     const at::Tensor& wu_, const OptTensor& bg_,
                     const OptTensor& bu_, int64_t act, double p, int64_t seed,
-                    int64_t offset, const OptTensor& offset_t_,
-                    const OptTensor& wg_grad, const OptTensor& wu_grad,
-                    const OptTensor& bg_grad, const OptTensor& bu_grad) {
+                    int64_t offset, const OptTensor& offset_t_) {
   const char* name = "gated_linear";
   for (auto* t : {&x_, &wg_, &wu_}) check_tangent(*t, name);
   for (auto* t : {&bg_, &bu_}) if (*t) check_tangent(**t, name);
@@ -191,7 +200,8 @@ at::Tensor gated_ad(const at::Tensor& x_, const at::Tensor& wg_,
        (bg && bg->requires_grad()) || (bu && bu->requires_grad())))
     return GatedFn::apply(
         x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
-        std::vector<OptTensor>{wg_grad, wu_grad, bg_grad, bu_grad});
+        std::vector<OptTensor>{grad_buffer(wg_), grad_buffer(wu_),
+                               grad_buffer(bg_), grad_buffer(bu_)});
   return gated_fwd(x, wg, wu, bg, bu, act, p, seed, offset, offset_t,
                    false)[0];
 }
@@ -199,21 +209,17 @@ at::Tensor gated_ad(const at::Tensor& x_, const at::Tensor& wg_,
 at::Tensor gated_call(const at::Tensor& x, const at::Tensor& wg,
                       const at::Tensor& wu, const OptTensor& bg,
                       const OptTensor& bu, int64_t act, double p,
-                      int64_t seed, int64_t offset, const OptTensor& offset_t,
-                      const std::vector<OptTensor>& outs) {
+                      int64_t seed, int64_t offset,
+                      const OptTensor& offset_t) {
   static const auto op =
       c10::Dispatcher::singleton().findSchemaOrThrow("dvgg::gated_linear", "")
           .typed<at::Tensor(const at::Tensor&, const at::Tensor&,
                             const at::Tensor&, const OptTensor&,
                             const OptTensor&, int64_t, double, int64_t,
-                            int64_t, const OptTensor&, const OptTensor&,
-                            const OptTensor&, const OptTensor&,
-                            const OptTensor&)>();
-  TORCH_CHECK(outs.size() == 4, "gated_linear: four gradient buffers or None");
+                            int64_t, const OptTensor&)>();
   for (auto* t : {&x, &wg, &wu}) check_memory(*t, "gated_linear");
   for (auto* t : {&bg, &bu}) if (*t) check_memory(**t, "gated_linear");
-  return op.call(x, wg, wu, bg, bu, act, p, seed, offset, offset_t, outs[0],
-                 outs[1], outs[2], outs[3]);
+  return op.call(x, wg, wu, bg, bu, act, p, seed, offset, offset_t);
 }
 
 // without a key: one kernel for every pass through the dispatcher, which
@@ -223,9 +229,7 @@ TORCH_LIBRARY(dvgg, m) {
         "Tensor? offset_t=None) -> Tensor", dropout_ad);
   m.def("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, "
         "Tensor? bias_gate, Tensor? bias_up, int act, float p, int seed, "
-        "int offset, Tensor? offset_t=None, Tensor? w_gate_grad=None, "
-        "Tensor? w_up_grad=None, Tensor? bias_gate_grad=None, "
-        "Tensor? bias_up_grad=None) -> Tensor", gated_ad);
+        "int offset, Tensor? offset_t=None) -> Tensor", gated_ad);
 }
 
 }  // namespace dvgg

@@ -41,8 +41,7 @@ at::Tensor dropout_call(const at::Tensor&, double, int64_t, int64_t,
 at::Tensor gated_call(const at::Tensor&, const at::Tensor&, const at::Tensor&,
                       const c10::optional<at::Tensor>&,
                       const c10::optional<at::Tensor>&, int64_t, double,
-                      int64_t, int64_t, const c10::optional<at::Tensor>&,
-                      const std::vector<c10::optional<at::Tensor>>&);
+                      int64_t, int64_t, const c10::optional<at::Tensor>&);
 
 // gated.hip
 std::vector<int64_t> gated_plan(int64_t, int64_t, int64_t, int64_t);
@@ -104,7 +103,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_linear", &dvgg::gated_call, py::arg("x"), py::arg("w_gate"),
         py::arg("w_up"), py::arg("bias_gate"), py::arg("bias_up"),
         py::arg("act"), py::arg("p"), py::arg("seed"), py::arg("offset"),
-        py::arg("offset_t"), py::arg("grad_outs"));
+        py::arg("offset_t") = c10::nullopt);
   m.def("gated_plan", &dvgg::gated_plan, py::arg("product"),
         py::arg("rows"), py::arg("cols"), py::arg("k_len"));
   m.def("lrn_fwd", &dvgg::lrn_fwd);

@@ -66,10 +66,7 @@ def gated_linear(x, w_gate, w_up, bias_gate=None, bias_up=None,
     on_device = isinstance(offset, torch.Tensor)
     h = native.ext().gated_linear(
         flat, w_gate, w_up, bias_gate, bias_up, _ACT_ID[act], max(p, 0.0),
-        seed, 0 if on_device else offset, offset if on_device else None,
-        # direct-grad: arena views attached by ArenaOptimizer
-        [getattr(t, "_dvgg_gbuf", None)
-         for t in (w_gate, w_up, bias_gate, bias_up)])
+        seed, 0 if on_device else offset, offset if on_device else None)
     return h if x.dim() == 2 else h.view(*x.shape[:-1], h.shape[-1])
 
 

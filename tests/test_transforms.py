@@ -1,6 +1,8 @@
 """Dropout and the gated unit under what torch does around an operator:
 recording a call and replaying it, function transforms."""
 
+import io
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -110,7 +112,7 @@ def dual_calls(dev):
     def gated(which):
         ts = [half[0], half[1], half[1].clone(), b.bfloat16(), b.bfloat16()]
         ts[which] = fwAD.make_dual(ts[which], torch.ones_like(ts[which]))
-        return ext.gated_linear(*ts, 0, 0.0, 0, 0, None, [None] * 4)
+        return ext.gated_linear(*ts, 0, 0.0, 0, 0, None)
     return [lambda: ext.dropout(fwAD.make_dual(x, x), 0.5, 1, 1)] + \
         [lambda i=i: gated(i) for i in range(5)]
 
@@ -181,8 +183,7 @@ def zero_calls(dev):
     flat = torch._efficientzerotensor((8,), dtype=torch.bfloat16, device=dev)
 
     def gated(x=w, g=w, u=w, b=None):
-        return ext.gated_linear(x, g, u, b, None, 0, 0.0, 0, 0, None,
-                                [None] * 4)
+        return ext.gated_linear(x, g, u, b, None, 0, 0.0, 0, 0, None)
     return [lambda: ext.dropout(zero, 0.5, 1, 1), lambda: gated(x=zero),
             lambda: gated(g=zero), lambda: gated(u=zero),
             lambda: gated(b=flat)]
@@ -249,7 +250,7 @@ def test_tensors_without_memory_are_refused(which, make):
             return ext.dropout(make(w), 0.5, 1, 0)
         if which == 7:
             return ext.dropout(w, 0.5, 1, 0, make(ts[5]))
-        return ext.gated_linear(*ts[:5], 0, 0.5, 0, 0, ts[5], [None] * 4)
+        return ext.gated_linear(*ts[:5], 0, 0.5, 0, 0, ts[5])
     with pytest.raises(RuntimeError, match="without memory"):
         call()
 
@@ -277,3 +278,31 @@ def test_calls_under_autocast():
         y, h = ops.dropout(x, 0.5, 1, 1), ops.gated_linear(x, wg, wu)
     assert torch.equal(y, ops.dropout(x, 0.5, 1, 1))
     assert torch.equal(h, ops.gated_linear(x, wg, wu))
+
+
+@gpu
+def test_traced_layer_of_an_arena_and_its_saved_form():
+    from distributed_vgg_f_amd.engine.arena import ArenaOptimizer
+    layer = hidden_fc(64, 40, "silu")
+    ArenaOptimizer(layer, torch.device(DEV))
+    x, dh = [torch.randn(9, n, device=DEV).bfloat16() for n in (64, 40)]
+    traced = torch.jit.trace(layer, x)
+    want = layer(x)
+    want.backward(dh)
+    names = [n for n, _ in layer.named_parameters()]
+    grads = {n: p._dvgg_gbuf.clone() for n, p in layer.named_parameters()}
+    for p in layer.parameters():
+        p.grad = None
+        p._dvgg_gbuf.zero_()
+    h = traced(x)
+    assert torch.equal(h, want)
+    h.backward(dh)
+    for n, p in layer.named_parameters():
+        assert torch.equal(p.grad, grads[n]), n
+        assert p.grad.data_ptr() == p._dvgg_gbuf.data_ptr(), n
+    assert len(names) == 4
+
+    file = io.BytesIO()
+    torch.jit.save(traced, file)
+    file.seek(0)
+    assert torch.equal(torch.jit.load(file)(x), want)
